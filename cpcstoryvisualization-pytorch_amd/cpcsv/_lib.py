@@ -227,6 +227,9 @@ SIGNATURES = {
     "cpcsv_thin4x4s2_wgrad": [_P, _P, _P, _P, _I, _I, _I, _I, _P],
     "cpcsv_layer_update": [_P, _P],
     "cpcsv_adam_chunk": [],
+    "cpcsv_scan_chunks": [_I],
+    "cpcsv_scan_fwd": [_P, _I, _L, _L, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
+    "cpcsv_scan_bwd": [_P, _I, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
     "cpcsv_set_deterministic": [_I],
     "cpcsv_abi_layout": [_I, C.POINTER(C.c_int), _I],
     "cpcsv_set_wgrad_linear": [_I],

@@ -1365,6 +1365,112 @@ class GruSeqFn(Function):
         return dgi, carry, dw, db, None, None
 
 
+# ------------------------------------------------------------------------------------------------
+# gated linear recurrence
+# ------------------------------------------------------------------------------------------------
+def _scan_args(p, h0, lengths, out_gate, rank):
+    """Checks of gated_scan / gated_scan_step -> H."""
+    k = 3 if out_gate else 2
+    if p.dim() != rank:
+        raise ValueError("p must have %d dimensions, got shape %s" % (rank, tuple(p.shape)))
+    if p.shape[-1] % k or (p.shape[-1] == 0):
+        raise ValueError("the last dimension of p holds %d equal column blocks (%s), got %d columns"
+                         % (k, "f | v | o" if out_gate else "f | v", p.shape[-1]))
+    dcode(p)                                       # TypeError unless fp32 / bf16
+    h = p.shape[-1] // k
+    if h0 is not None:
+        if h0.dtype != torch.float32:
+            raise TypeError("the state is held in float32, got %s" % h0.dtype)
+        if tuple(h0.shape) != (p.shape[0], h):
+            raise ValueError("the state must have shape %s, got %s" % ((p.shape[0], h), tuple(h0.shape)))
+    if lengths is not None:
+        if lengths.dtype != torch.int32:
+            raise TypeError("lengths must be int32, got %s" % lengths.dtype)
+        if tuple(lengths.shape) != (p.shape[0],):
+            raise ValueError("lengths must have shape (%d,), got %s" % (p.shape[0], tuple(lengths.shape)))
+    _runtime.require_here(p, h0, lengths)
+    return h
+
+
+class GatedScanFn(Function):
+    """(y, h_last) of the gated linear recurrence; see gated_scan."""
+
+    @staticmethod
+    def forward(ctx, p, h0, lengths, out_gate):
+        b, t, h = p.shape[0], p.shape[1], p.shape[2] // (3 if out_gate else 2)
+        if p.stride(2) != 1:
+            p = p.contiguous()
+        h0 = h0.contiguous() if h0 is not None else None
+        lengths = lengths.contiguous() if lengths is not None else None
+        dev = p.device
+        y = _empty((b, t, h), p.dtype, dev)
+        last = _empty((b, h), torch.float32, dev)
+        hin = None
+        if b == 0 or t == 0:
+            last.copy_(h0) if h0 is not None else last.zero_()
+        else:
+            nc = K.scan_chunks(t)
+            sA = None
+            if nc > 1:
+                hin, sA = _empty((b, nc, h), torch.float32, dev), _empty((b, nc, h), torch.float32, dev)
+            K.scan_fwd(p, h0, lengths, y, last, hin, sA, b, t, h, out_gate)
+            _runtime.keep_forced(p, h0, lengths, hin, sA)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(p, h0, lengths, hin)
+        ctx.out_gate = out_gate
+        return y, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dlast):
+        p, h0, lengths, hin = ctx.saved_tensors
+        b, t, h = p.shape[0], p.shape[1], p.shape[2] // (3 if ctx.out_gate else 2)
+        if dy is None and dlast is None:
+            return None, None, None, None
+        dev = p.device
+        dp = _empty(p.shape, p.dtype, dev)
+        dh0 = _empty((b, h), torch.float32, dev) if h0 is not None and ctx.needs_input_grad[1] else None
+        if b == 0 or t == 0:
+            if dh0 is not None:
+                dh0.copy_(dlast) if dlast is not None else dh0.zero_()
+            return dp, dh0, None, None
+        dy = torch.zeros((b, t, h), dtype=p.dtype, device=dev) if dy is None else dy.contiguous()
+        dlast = dlast.contiguous() if dlast is not None else None
+        sA = sC = None
+        if hin is not None:
+            sA, sC = _empty(hin.shape, torch.float32, dev), _empty(hin.shape, torch.float32, dev)
+        K.scan_bwd(p, h0, lengths, hin, dy, dlast, dp, dh0, sA, sC, b, t, h, ctx.out_gate)
+        _runtime.keep_forced(dy, dlast, sA, sC)
+        return dp, dh0, None, None
+
+
+def gated_scan(p, h0=None, lengths=None, out_gate=True):
+    """Gated linear recurrence over a packed projection p [B, T, 3H] with columns f | v | o (fp32 or bf16; any strides of B and T):
+        z_t = sigmoid(f_t);  h_t = z_t h_{t-1} + (1 - z_t) v_t;  y_t = h_t silu(o_t)
+    out_gate=False: p is [B, T, 2H] and y_t = h_t. h0 fp32 [B, H] (None: zeros). lengths int32 [B]: a sequence ends there - what stands
+    behind it in p is not read, its y and gradient are zero, and its last state is the one at the end (length 0: h0).
+    -> (y [B, T, H] in p's type, h_last fp32 [B, H]). Differentiable in p and h0, once. The GRU's gate convention (modules.GRUCell)
+    without W_hh: the whole sequence is three launches however long it is."""
+    _scan_args(p, h0, lengths, out_gate, 3)
+    return GatedScanFn.apply(p, h0, lengths, bool(out_gate))
+
+
+@torch.no_grad()
+def gated_scan_step(p, h, out_gate=True):
+    """One token of gated_scan for every row: p [B, 3H] (2H without the output gate), h fp32 [B, H] contiguous, UPDATED IN PLACE.
+    -> y [B, H] in p's type. One launch, nothing allocated but y; for generation (no gradients)."""
+    hid = _scan_args(p, h, None, out_gate, 2)
+    if h is None or not h.is_contiguous():
+        raise ValueError("the state is updated in place: it must be a contiguous tensor")
+    if p.stride(1) != 1:
+        p = p.contiguous()
+    y = _empty((p.shape[0], hid), p.dtype, p.device)
+    if p.shape[0]:
+        K.scan_fwd(p.unsqueeze(1), h, None, y, h, None, None, p.shape[0], 1, hid, out_gate)
+        _runtime.keep_forced(p)
+    return y
+
+
 class DynFilter1dFn(Function):
     """DynamicFilterLayer1D.forward (layers.py:69-80) as one launch: sig (N,C,L), taps (N,1,C,K) -> (N,1,L)."""
 

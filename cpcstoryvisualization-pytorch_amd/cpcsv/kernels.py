@@ -602,3 +602,17 @@ def batch_prep(im_desc, im_lab, im_cont, st_desc, st_lab, td):
     _call("cpcsv_batch_prep", ptr(im_desc), im_desc.stride(0), ptr(im_lab), ptr(im_cont), im_cont.stride(1), ptr(st_desc), st_desc.stride(1),
           ptr(st_lab), ptr(im_motion), ptr(im_content), ptr(st_motion), ptr(st_text), ptr(st_mean), ptr(chars), im, st, t, td, l, stream())
     return im_motion, im_content, st_motion, st_text, st_mean, chars
+
+
+def scan_chunks(T):
+    return L.load().cpcsv_scan_chunks(T)
+
+
+def scan_fwd(p, h0, lengths, y, h_last, hin, sA, B, T, H, out_gate):
+    _call("cpcsv_scan_fwd", ptr(p), dcode(p), p.stride(0), p.stride(1), ptr(h0), ptr(lengths), ptr(y), ptr(h_last), ptr(hin), ptr(sA),
+          B, T, H, int(out_gate), stream())
+
+
+def scan_bwd(p, h0, lengths, hin, dy, dh_last, dp, dh0, sA, sC, B, T, H, out_gate):
+    _call("cpcsv_scan_bwd", ptr(p), dcode(p), p.stride(0), p.stride(1), ptr(h0), ptr(lengths), ptr(hin), ptr(dy), ptr(dh_last), ptr(dp),
+          ptr(dh0), ptr(sA), ptr(sC), B, T, H, int(out_gate), stream())

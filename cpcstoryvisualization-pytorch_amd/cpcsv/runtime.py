@@ -375,5 +375,22 @@ def require_gpu(t):
                            "There is no CPU fallback in the product path." % t.device)
 
 
+def require_here(*tensors):
+    """Every tensor (None is skipped) is on the current GPU: kernels go to the current device's stream."""
+    for t in tensors:
+        if t is not None:
+            require_gpu(t)
+            if t.get_device() != _current_device():
+                raise RuntimeError("tensor on %s while the current device is cuda:%d: call inside `with torch.cuda.device(...)`"
+                                   % (t.device, _current_device()))
+
+
+def keep_forced(*tensors):
+    """Scratch that a call allocates and drops: under `forced_stream` its kernels run on another stream than the allocator's current
+    one, so it has to outlive them (until release_kept())."""
+    if _FORCED[0] is not None:
+        keep_alive(*tensors)
+
+
 if os.environ.get("CPCSV_DETERMINISTIC", "0") == "1":
     set_deterministic(True)

@@ -725,6 +725,24 @@ int cpcsv_thin4x4s2_dgrad(const void* dz, const void* w_bwd, void* dx, const flo
 int cpcsv_thin4x4s2_wgrad_slabs(int N, int H, int W);
 int cpcsv_thin4x4s2_wgrad(const void* dz, const void* x, float* G, float* slabs, int N, int H, int W, int Cout, void* stream);
 
+/* ---- gated linear recurrence (csrc/scan.hip) -----------------------------------------------------------------------
+ * Stands beside the GRU entry points above (reference model.py:223-224,316-341): the same gate convention without the
+ * state's product, so that the time axis can be split.
+ *   z = sigmoid(f_t)   h_t = z h_{t-1} + (1 - z) v_t   y_t = h_t * silu(o_t)  (out_gate == 0: y_t = h_t)
+ *   p        [B][T][3H] (2H without out_gate), columns f | v | o, dtype; psb / pst = element strides of b / t, unit stride in a row
+ *   h0       fp32 [B][H] or NULL (zeros); h_last fp32 [B][H] or NULL: the state behind the last token. With T == 1 h_last may be h0
+ *   lengths  int32 [B] on the device or NULL (all T; values are clamped to 0..T): tokens behind a sequence's end are not read, their
+ *            y and dp are zero, and h_last is the state at the sequence's end
+ *   y, dy    [B][T][H] dtype, contiguous; dp [B][T][3H or 2H] dtype, contiguous; dh_last, dh0 fp32 [B][H] or NULL
+ *   hin, sA, sC  fp32 [B][cpcsv_scan_chunks(T)][H] workspaces, needed when that count is above 1 (else NULL): hin is filled by the
+ *            forward call and read by the backward call of the same inputs, the others are scratch
+ * No atomics: results do not depend on the run. */
+int cpcsv_scan_chunks(int T);
+int cpcsv_scan_fwd(const void* p, int dtype, long psb, long pst, const float* h0, const int* lengths, void* y, float* h_last,
+                   float* hin, float* sA, int B, int T, int H, int out_gate, void* stream);
+int cpcsv_scan_bwd(const void* p, int dtype, long psb, long pst, const float* h0, const int* lengths, const float* hin, const void* dy,
+                   const float* dh_last, void* dp, float* dh0, float* sA, float* sC, int B, int T, int H, int out_gate, void* stream);
+
 /* Reproducible mode (tests, debugging): 1 = every cross-block floating-point reduction runs in ONE fixed order (weight
  * gradients without pixel splits, BatchNorm/spectral-norm/bias sums without contended atomics), so two runs of the same
  * step - eager or replayed from a HIP graph - give bit-identical results. Process-wide; returns the previous setting.
