@@ -230,12 +230,18 @@ SIGNATURES = {
     "cpcsv_scan_chunks": [_I],
     "cpcsv_scan_fwd": [_P, _I, _L, _L, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
     "cpcsv_scan_bwd": [_P, _I, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
+    "cpcsv_norm_residual_fwd": [_P] * 10 + [_L, _I, _I, _I, _I, _L, _F, _P],
+    "cpcsv_norm_residual_part": [_L, _I, _I, _L],
+    "cpcsv_norm_residual_bwd": [_P] * 17 + [_L, _I, _I, _I, _I, _L, _P],
     "cpcsv_set_deterministic": [_I],
     "cpcsv_abi_layout": [_I, C.POINTER(C.c_int), _I],
     "cpcsv_set_wgrad_linear": [_I],
     "cpcsv_version": [],
     "cpcsv_arch": [],
 }
+
+_LONG = ("cpcsv_logit_head_scratch", "cpcsv_norm_residual_part")        # entry points that return a count as long
+NORM_MAX_D = 16384         # CPCSV_NORM_MAX_D
 
 _lib = None
 
@@ -287,7 +293,7 @@ def load():
     for name, args in SIGNATURES.items():
         fn = getattr(lib, name)  # AttributeError if the symbol is missing
         fn.argtypes = args
-        fn.restype = C.c_char_p if name == "cpcsv_arch" else (C.c_long if name == "cpcsv_logit_head_scratch" else C.c_int)
+        fn.restype = C.c_char_p if name == "cpcsv_arch" else (C.c_long if name in _LONG else C.c_int)
     verify_layout(lib)
     _lib = lib
     return lib

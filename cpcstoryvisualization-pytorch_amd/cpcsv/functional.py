@@ -1471,6 +1471,125 @@ def gated_scan_step(p, h, out_gate=True):
     return y
 
 
+# ------------------------------------------------------------------------------------------------
+# norms around a block
+# ------------------------------------------------------------------------------------------------
+class NormResidualFn(Function):
+    """Forward / backward of norm_residual and rms_norm (u None). x, u, gate: contiguous; gate [samples, D] or shaped like u."""
+
+    @staticmethod
+    def forward(ctx, x, u, w_post, gate, scale, w_next, out_dtype, eps):
+        d = x.shape[-1]
+        rows = x.numel() // d if d else 0
+        dev, udt = x.device, dcode(u) if u is not None else (L.F32 if out_dtype == torch.float32 else L.BF16)
+        x = x.contiguous()
+        u, gate = (None if q is None else q.contiguous() for q in (u, gate))
+        w_post, scale, w_next = (None if q is None else q.contiguous() for q in (w_post, scale, w_next))
+        mode, t = 0, 1
+        if gate is not None:
+            per = gate.numel() // d if d else 0
+            mode, t = (1, 1) if per == rows else (2, rows // per)
+        xo = _empty(x.shape, x.dtype, dev) if u is not None else None
+        z = _empty(x.shape, out_dtype, dev) if w_next is not None else None
+        ru = rx = None
+        if rows:
+            ru = _empty((rows,), torch.float32, dev) if u is not None else None
+            rx = _empty((rows,), torch.float32, dev) if w_next is not None else None
+            K.norm_residual_fwd(x, u, gate, scale, w_post, w_next, xo, z, ru, rx, rows, d, udt, mode, t, eps)
+            _runtime.keep_forced(x, u, gate, w_post, scale, w_next, ru, rx)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, u, w_post, gate, scale, w_next, ru, rx)
+        ctx.geom = (rows, d, udt, mode, t)
+        return (xo, z) if xo is not None and z is not None else (xo if xo is not None else z)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        x, u, w_post, gate, scale, w_next, ru, rx = ctx.saved_tensors
+        rows, d, udt, mode, t = ctx.geom
+        if len(grads) == 2:
+            dxo, dz = grads
+        else:
+            dxo, dz = (grads[0], None) if u is not None else (None, grads[0])
+        if dxo is None and dz is None:
+            return (None,) * 8
+        need = ctx.needs_input_grad
+        dev, f32 = x.device, torch.float32
+        like = lambda q, on: _empty(q.shape, q.dtype, dev) if (on and q is not None) else None
+        dx, du, dgate = _empty(x.shape, x.dtype, dev), like(u, need[1]), like(gate, need[3])
+        dwp, dsc, dwn = like(w_post, need[2]), like(scale, need[4]), like(w_next, need[5])
+        if not rows:
+            for q in (dwp, dsc, dwn, dgate):
+                if q is not None:
+                    q.zero_()
+            return dx, du, dwp, dgate, dsc, dwn, None, None
+        dxo = dxo.contiguous() if dxo is not None else None
+        dz = dz.contiguous() if dz is not None else None
+        if dz is None and dwn is not None:
+            dwn.zero_()
+        part = None
+        if dwp is not None or dsc is not None or dwn is not None or (mode == 2 and dgate is not None):
+            part = _empty((K.norm_residual_part(rows, d, mode, t),), f32, dev)
+        K.norm_residual_bwd(x, u, gate, scale, w_post, w_next, ru, rx, dxo, dz, dx, du, dgate, dsc, dwp, dwn, part, rows, d, udt, mode, t)
+        _runtime.keep_forced(dxo, dz, part)
+        return dx, du, dwp, dgate, dsc, dwn, None, None
+
+
+def _norm_vec(name, w, d):
+    if w.dtype != torch.float32:
+        raise TypeError("%s must be float32, got %s" % (name, w.dtype))
+    if tuple(w.shape) != (d,):
+        raise ValueError("%s must have shape (%d,), got %s" % (name, d, tuple(w.shape)))
+
+
+def _norm_x(x):
+    dcode(x)
+    if x.dim() < 1 or x.shape[-1] < 1 or x.shape[-1] > L.NORM_MAX_D:
+        raise ValueError("rows of 1..%d values expected, got shape %s" % (L.NORM_MAX_D, tuple(x.shape)))
+    return x.shape[-1]
+
+
+def rms_norm(x, weight, eps=1e-6, out_dtype=None):
+    """weight * x / sqrt(mean x^2 + eps) over the last dimension (fp32 or bf16 x, fp32 weight [D], D <= 16384), statistics in fp32.
+    out_dtype: the result's type (default x's; bf16 from an fp32 residual stream feeds the compute dtype). The norm before the first
+    block; norm_residual holds those behind it."""
+    d = _norm_x(x)
+    _norm_vec("weight", weight, d)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in (torch.float32, torch.bfloat16) or (x.dtype == torch.bfloat16 and out_dtype == torch.float32):
+        raise TypeError("out_dtype must be x's type or bfloat16, got %s of %s" % (out_dtype, x.dtype))
+    _runtime.require_here(x, weight)
+    return NormResidualFn.apply(x, None, None, None, None, weight, out_dtype, float(eps))
+
+
+def norm_residual(x, u, w_post, gate=None, scale=None, w_next=None, eps=1e-6):
+    """The norm behind a block, its gate, its residual scale, the residual sum, and the norm before the next block in one pass:
+        x' = x + scale * gate * w_post * u / rms(u);    z = w_next * x' / rms(x');    rms(a) = sqrt(mean a^2 + eps)
+    x [..., D]: the residual stream (fp32 or bf16). u, like x: the block's output (x's type, or bf16 with an fp32 stream).
+    gate: None, u's shape (one a token), or [B, 1, ..., 1, D] / [B, D] with B = x.shape[0] (one a sample, its gradient summed over
+    the sample's tokens); u's type. scale, w_post, w_next: fp32 [D]. -> (x', z), or x' alone when w_next is None; x' in x's type, z in
+    u's. z is formed from x' before it is rounded. Differentiable once in every tensor."""
+    d = _norm_x(x)
+    dcode(u)
+    if x.dtype == torch.bfloat16 and u.dtype != torch.bfloat16:
+        raise TypeError("u must be bfloat16 on a bfloat16 residual stream, got %s" % u.dtype)
+    if u.shape != x.shape:
+        raise ValueError("u must have x's shape %s, got %s" % (tuple(x.shape), tuple(u.shape)))
+    for name, w in (("w_post", w_post), ("scale", scale), ("w_next", w_next)):
+        if w is not None:
+            _norm_vec(name, w, d)
+    if gate is not None:
+        if gate.dtype != u.dtype:
+            raise TypeError("gate must have u's type %s, got %s" % (u.dtype, gate.dtype))
+        b = x.shape[0]
+        if gate.shape != x.shape and tuple(gate.shape) not in ((b, d), (b,) + (1,) * (x.dim() - 2) + (d,)):
+            raise ValueError("gate must have u's shape %s or one row a sample (%d, ..., %d), got %s" % (tuple(u.shape), b, d, tuple(gate.shape)))
+        if x.dim() == 1:
+            raise ValueError("a gate needs x of at least two dimensions")
+    _runtime.require_here(x, u, w_post, gate, scale, w_next)
+    return NormResidualFn.apply(x, u, w_post, gate, scale, w_next, u.dtype, float(eps))
+
+
 class DynFilter1dFn(Function):
     """DynamicFilterLayer1D.forward (layers.py:69-80) as one launch: sig (N,C,L), taps (N,1,C,K) -> (N,1,L)."""
 

@@ -616,3 +616,18 @@ def scan_fwd(p, h0, lengths, y, h_last, hin, sA, B, T, H, out_gate):
 def scan_bwd(p, h0, lengths, hin, dy, dh_last, dp, dh0, sA, sC, B, T, H, out_gate):
     _call("cpcsv_scan_bwd", ptr(p), dcode(p), p.stride(0), p.stride(1), ptr(h0), ptr(lengths), ptr(hin), ptr(dy), ptr(dh_last), ptr(dp),
           ptr(dh0), ptr(sA), ptr(sC), B, T, H, int(out_gate), stream())
+
+
+def norm_residual_fwd(x, u, gate, scale, w_post, w_next, xo, z, ru, rx, rows, D, udt, gate_mode, T, eps):
+    _call("cpcsv_norm_residual_fwd", ptr(x), ptr(u), ptr(gate), ptr(scale), ptr(w_post), ptr(w_next), ptr(xo), ptr(z), ptr(ru), ptr(rx),
+          rows, D, dcode(x), udt, gate_mode, T, float(eps), stream())
+
+
+def norm_residual_part(rows, D, gate_mode, T):
+    return L.load().cpcsv_norm_residual_part(rows, D, gate_mode, T)
+
+
+def norm_residual_bwd(x, u, gate, scale, w_post, w_next, ru, rx, dxo, dz, dx, du, dgate, dscale, dw_post, dw_next, part, rows, D, udt,
+                      gate_mode, T):
+    _call("cpcsv_norm_residual_bwd", ptr(x), ptr(u), ptr(gate), ptr(scale), ptr(w_post), ptr(w_next), ptr(ru), ptr(rx), ptr(dxo), ptr(dz),
+          ptr(dx), ptr(du), ptr(dgate), ptr(dscale), ptr(dw_post), ptr(dw_next), ptr(part), rows, D, dcode(x), udt, gate_mode, T, stream())

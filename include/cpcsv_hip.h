@@ -743,6 +743,26 @@ int cpcsv_scan_fwd(const void* p, int dtype, long psb, long pst, const float* h0
 int cpcsv_scan_bwd(const void* p, int dtype, long psb, long pst, const float* h0, const int* lengths, const float* hin, const void* dy,
                    const float* dh_last, void* dp, float* dh0, float* sA, float* sC, int B, int T, int H, int out_gate, void* stream);
 
+/* ---- norms around a block, fused with its gate and residual scale (csrc/blocknorm.hip) --------------------------------
+ * Stands beside the BatchNorm entry points: root-mean-square norms over the D values of each row, no batch statistics.
+ *   uh = u / rms(u)    xo = x + scale * gate * w_post * uh    z = w_next * xo / rms(xo)     rms(a) = sqrt(mean a^2 + eps)
+ *   x, xo    [rows][D] xdt, the residual stream    u, z, gate [rows][D] udt; (xdt, udt) = both fp32, both bf16, or fp32 with bf16.
+ *   u NULL: z = w_next * x / rms(x) alone (xo, gate, scale, w_post unused); w_next NULL: no z.
+ *   gate_mode  0 none, 1 one row for each row, 2 gate [rows / T][D]: one row for T consecutive rows (T divides rows)
+ *   scale, w_post, w_next  fp32 [D]; scale NULL = 1        ru, rx  fp32 [rows]: 1/rms, written forward, read backward
+ *   dxo (NULL = 0), dx xdt; dz (NULL = 0), du, dgate udt; dscale, dw_post, dw_next fp32 [D]; each result but dx may be NULL
+ *   part     fp32 workspace of cpcsv_norm_residual_part(...) values, needed when a weight's or a shared gate's gradient is asked for
+ * D up to CPCSV_NORM_MAX_D. Contiguous tensors. No atomics: results do not depend on the run. */
+#define CPCSV_NORM_MAX_D 16384
+int cpcsv_norm_residual_fwd(const void* x, const void* u, const void* gate, const float* scale, const float* w_post, const float* w_next,
+                            void* xo, void* z, float* ru, float* rx, long rows, int D, int xdt, int udt, int gate_mode, long T, float eps,
+                            void* stream);
+long cpcsv_norm_residual_part(long rows, int D, int gate_mode, long T);
+int cpcsv_norm_residual_bwd(const void* x, const void* u, const void* gate, const float* scale, const float* w_post, const float* w_next,
+                            const float* ru, const float* rx, const void* dxo, const void* dz, void* dx, void* du, void* dgate,
+                            float* dscale, float* dw_post, float* dw_next, float* part, long rows, int D, int xdt, int udt, int gate_mode,
+                            long T, void* stream);
+
 /* Reproducible mode (tests, debugging): 1 = every cross-block floating-point reduction runs in ONE fixed order (weight
  * gradients without pixel splits, BatchNorm/spectral-norm/bias sums without contended atomics), so two runs of the same
  * step - eager or replayed from a HIP graph - give bit-identical results. Process-wide; returns the previous setting.
