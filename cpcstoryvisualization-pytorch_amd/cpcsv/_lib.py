@@ -233,6 +233,9 @@ SIGNATURES = {
     "cpcsv_norm_residual_fwd": [_P] * 10 + [_L, _I, _I, _I, _I, _L, _F, _P],
     "cpcsv_norm_residual_part": [_L, _I, _I, _L],
     "cpcsv_norm_residual_bwd": [_P] * 17 + [_L, _I, _I, _I, _I, _L, _P],
+    "cpcsv_orth_workspace": [_P, _I],
+    "cpcsv_orthogonalize": [_P, _P, _P, _I, _I, _I, _F, _P, _P],
+    "cpcsv_muon_step": [_P, _P, _P, _P, _I, _P, _F, _I, _F, _I, _F, _P, _P],
     "cpcsv_set_deterministic": [_I],
     "cpcsv_abi_layout": [_I, C.POINTER(C.c_int), _I],
     "cpcsv_set_wgrad_linear": [_I],
@@ -240,8 +243,9 @@ SIGNATURES = {
     "cpcsv_arch": [],
 }
 
-_LONG = ("cpcsv_logit_head_scratch", "cpcsv_norm_residual_part")        # entry points that return a count as long
+_LONG = ("cpcsv_logit_head_scratch", "cpcsv_norm_residual_part", "cpcsv_orth_workspace")        # entry points that return a count as long
 NORM_MAX_D = 16384         # CPCSV_NORM_MAX_D
+ORTH_JOBS, ORTH_MAX_SIDE = 16, 131072          # CPCSV_ORTH_JOBS, CPCSV_ORTH_MAX_SIDE
 
 _lib = None
 

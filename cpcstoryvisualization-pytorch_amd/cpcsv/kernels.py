@@ -631,3 +631,35 @@ def norm_residual_bwd(x, u, gate, scale, w_post, w_next, ru, rx, dxo, dz, dx, du
                       gate_mode, T):
     _call("cpcsv_norm_residual_bwd", ptr(x), ptr(u), ptr(gate), ptr(scale), ptr(w_post), ptr(w_next), ptr(ru), ptr(rx), ptr(dxo), ptr(dz),
           ptr(dx), ptr(du), ptr(dgate), ptr(dscale), ptr(dw_post), ptr(dw_next), ptr(part), rows, D, dcode(x), udt, gate_mode, T, stream())
+
+
+def _orth_lists(*lists):
+    """HOST arrays of the matrices' device pointers."""
+    return [(C.c_void_p * len(ts))(*[t.data_ptr() for t in ts]) for ts in lists]
+
+
+def _orth_ws(shapes, dev):
+    dims = (C.c_long * (2 * len(shapes)))(*[v for s in shapes for v in s])
+    n = L.load().cpcsv_orth_workspace(dims, len(shapes))
+    if n < 0:
+        raise RuntimeError("cpcsv_orth_workspace failed with code %d" % n)
+    ws = torch.empty(n // 2, dtype=torch.float16, device=dev)
+    if _os.environ.get("CPCSV_POISON", "0") == "1":
+        ws.fill_(float("nan"))
+    return dims, ws
+
+
+def orthogonalize(gs, outs, shapes, steps, eps):
+    """Up to L.ORTH_JOBS contiguous matrices of one type in shared launches (cpcsv_orthogonalize); returns the workspace."""
+    dims, ws = _orth_ws(shapes, gs[0].device)
+    g, o = _orth_lists(gs, outs)
+    _call("cpcsv_orthogonalize", g, o, dims, len(gs), dcode(gs[0]), steps, float(eps), ptr(ws), stream())
+    return ws
+
+
+def muon_step(weights, grads, moms, shapes, hyper, momentum, nesterov, decay, steps, eps):
+    """Up to L.ORTH_JOBS matrices in shared launches (cpcsv_muon_step); returns the workspace."""
+    dims, ws = _orth_ws(shapes, weights[0].device)
+    w, g, m = _orth_lists(weights, grads, moms)
+    _call("cpcsv_muon_step", w, g, m, dims, len(weights), ptr(hyper), float(momentum), int(nesterov), float(decay), steps, float(eps), ptr(ws), stream())
+    return ws

@@ -11,6 +11,7 @@ import torch
 
 from . import _lib as L
 from . import kernels as K
+from . import runtime as R
 from .runtime import dcode
 
 
@@ -276,4 +277,113 @@ class FusedAdam(torch.optim.Optimizer):
                 p._cpcsv_epoch = getattr(p, "_cpcsv_epoch", 0) + 1
             if gi == 0 and self._layers:
                 self._step_layers(group, hyper, pending, gscale, wire_of)        # reads the step count the launch above just advanced
+        return loss
+
+
+def _side_ok(shape, what):
+    if min(shape) < 1 or max(shape) > L.ORTH_MAX_SIDE:
+        raise ValueError("%s: sides of 1..%d expected, got %s" % (what, L.ORTH_MAX_SIDE, tuple(shape)))
+
+
+@torch.no_grad()
+def orthogonalize(g, steps=5, eps=1e-7):
+    """g [rows, cols] or a stack [n, rows, cols] (fp32 or bf16) with its singular values taken towards 1 (between 0.7 and 1.2 after
+    five steps) and its singular vectors kept: X = g / (|g|_F + eps), `steps` quintic Newton-Schulz products, as many launches for a stack of
+    up to 16 as for one matrix. -> a new tensor of g's type. An all-zero matrix stays zero. No gradient. cpcsv.optim.FusedMuon is the
+    optimiser around it."""
+    if g.dim() not in (2, 3):
+        raise ValueError("orthogonalize expects [rows, cols] or [n, rows, cols], got shape %s" % (tuple(g.shape),))
+    dcode(g)
+    if int(steps) != steps or steps < 1:
+        raise ValueError("steps must be a positive whole number, got %r" % (steps,))
+    if not eps >= 0:
+        raise ValueError("eps must not be negative, got %r" % (eps,))
+    _side_ok(g.shape[-2:], "orthogonalize")
+    R.require_here(g)
+    src = g.contiguous()
+    out = torch.empty_like(src)
+    one = (lambda t: list(t)) if g.dim() == 3 else (lambda t: [t])
+    gs, outs = one(src), one(out)
+    for i in range(0, len(gs), L.ORTH_JOBS):
+        part = gs[i:i + L.ORTH_JOBS]
+        ws = K.orthogonalize(part, outs[i:i + L.ORTH_JOBS], [tuple(q.shape) for q in part], int(steps), eps)
+        R.keep_forced(src, out, ws)
+    return out
+
+
+class FusedMuon(torch.optim.Optimizer):
+    """Momentum, orthogonalised: for weights that act as matrices (dense, convolution - seen as [out, inputs x taps] -, recurrent).
+        m <- momentum m + g;  U = g + momentum m (nesterov) or m;  X = orthogonalize(U);
+        w <- w (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) X
+    Up to 16 matrices share each of the 3 steps + 2 launches (csrc/orth.hip); biases, norms and other vectors belong to FusedAdam. Like
+    there the learning rate lives on the device (graph replays follow sync_lr()), operand caches of the weights are invalidated, and
+    parameters, gradients and momentum are contiguous fp32 GPU tensors."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, eps=1e-7):
+        if not lr >= 0 or not 0 <= momentum < 1 or not weight_decay >= 0 or not eps >= 0:
+            raise ValueError("FusedMuon: lr, weight_decay and eps must not be negative, momentum lies in [0, 1)")
+        if int(steps) != steps or steps < 1:
+            raise ValueError("FusedMuon: steps must be a positive whole number, got %r" % (steps,))
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=int(steps), eps=eps))
+        self._hypers = {}
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() < 2:
+                raise ValueError("FusedMuon takes matrices (two or more dimensions), got shape %s: leave vectors to FusedAdam" % (tuple(p.shape),))
+            _side_ok(self._matrix(p), "FusedMuon")
+
+    @staticmethod
+    def _matrix(p):
+        return p.shape[0], (p.numel() // p.shape[0] if p.shape[0] else 0)
+
+    def _hyper(self, gi, group, dev):
+        h = self._hypers.get(gi)
+        if h is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("FusedMuon: run one step before capturing one (its device scalars are made there)")
+            h = self._hypers[gi] = [torch.tensor([float(group["lr"])], dtype=torch.float32, device=dev), group["lr"]]
+        elif h[1] != group["lr"]:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("learning rate changed during graph capture")
+            h[0].fill_(float(group["lr"]))
+            h[1] = group["lr"]
+        return h[0]
+
+    def sync_lr(self):
+        """Push host-side lr changes to the device scalars (call after editing param_groups when using HIP graphs)."""
+        for gi, group in enumerate(self.param_groups):
+            if gi in self._hypers and self._hypers[gi][1] != group["lr"]:
+                self._hypers[gi][0].fill_(float(group["lr"]))
+                self._hypers[gi][1] = group["lr"]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for gi, group in enumerate(self.param_groups):
+            plist = [p for p in group["params"] if p.grad is not None]
+            for p in plist:
+                st = self.state[p]
+                ok = lambda t: t.is_cuda and t.dtype == torch.float32 and t.is_contiguous() and t.shape == p.shape
+                if not ok(p) or not ok(p.grad):
+                    raise RuntimeError("FusedMuon needs contiguous fp32 GPU parameters and gradients")
+                if "momentum_buffer" not in st:
+                    st["momentum_buffer"] = torch.zeros_like(p)
+                elif not ok(st["momentum_buffer"]):
+                    raise RuntimeError("FusedMuon needs contiguous fp32 GPU momentum of the parameter's shape")
+                R.require_here(p, p.grad, st["momentum_buffer"])
+            if not plist:
+                continue
+            hyper = self._hyper(gi, group, plist[0].device)
+            for i in range(0, len(plist), L.ORTH_JOBS):
+                part = plist[i:i + L.ORTH_JOBS]
+                ws = K.muon_step(part, [p.grad for p in part], [self.state[p]["momentum_buffer"] for p in part], [self._matrix(p) for p in part],
+                                 hyper, group["momentum"], group["nesterov"], group["weight_decay"], group["steps"], group["eps"])
+                R.keep_forced(ws)
+            for p in plist:      # invalidate packed-operand caches (cpcsv.modules.KernelLayer.packs)
+                p._cpcsv_epoch = getattr(p, "_cpcsv_epoch", 0) + 1
         return loss
