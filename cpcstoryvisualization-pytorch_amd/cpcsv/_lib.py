@@ -245,7 +245,7 @@ SIGNATURES = {
 
 _LONG = ("cpcsv_logit_head_scratch", "cpcsv_norm_residual_part", "cpcsv_orth_workspace")        # entry points that return a count as long
 NORM_MAX_D = 16384         # CPCSV_NORM_MAX_D
-ORTH_JOBS, ORTH_MAX_SIDE = 16, 131072          # CPCSV_ORTH_JOBS, CPCSV_ORTH_MAX_SIDE
+ORTH_JOBS, ORTH_MAX_SIDE, ORTH_MAX_MIN = 16, 131072, 16384         # CPCSV_ORTH_JOBS, CPCSV_ORTH_MAX_SIDE, CPCSV_ORTH_MAX_MIN
 
 _lib = None
 

@@ -281,8 +281,8 @@ class FusedAdam(torch.optim.Optimizer):
 
 
 def _side_ok(shape, what):
-    if min(shape) < 1 or max(shape) > L.ORTH_MAX_SIDE:
-        raise ValueError("%s: sides of 1..%d expected, got %s" % (what, L.ORTH_MAX_SIDE, tuple(shape)))
+    if min(shape) < 1 or max(shape) > L.ORTH_MAX_SIDE or min(shape) > L.ORTH_MAX_MIN:
+        raise ValueError("%s: sides of 1..%d expected, the shorter one up to %d, got %s" % (what, L.ORTH_MAX_SIDE, L.ORTH_MAX_MIN, tuple(shape)))
 
 
 @torch.no_grad()

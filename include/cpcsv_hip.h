@@ -767,7 +767,7 @@ int cpcsv_norm_residual_bwd(const void* x, const void* u, const void* gate, cons
  * Stands beside cpcsv_adam_step (reference trainer.py:212-220 uses Adam for every net): an optimiser for matrices.
  *   X = U / (|U|_F + eps), then `steps` times  A = X X^T, X <- a X + (b A + c A^2) X  with (a, b, c) = (3.4445, -4.7750, 2.0315),
  *   on the transpose where rows > cols. Results have the accuracy of fp32 products (two fp16 planes per operand, fp32 sums).
- * dims   HOST array [njobs][2] of rows, cols (1..CPCSV_ORTH_MAX_SIDE each); njobs in 1..CPCSV_ORTH_JOBS matrices share each launch
+ * dims   HOST array [njobs][2] of rows, cols (1..CPCSV_ORTH_MAX_SIDE each, the shorter one up to CPCSV_ORTH_MAX_MIN); njobs in 1..CPCSV_ORTH_JOBS matrices share each launch
  * ws     device workspace of cpcsv_orth_workspace(dims, njobs) bytes, 16-byte aligned, contents irrelevant before and after
  * cpcsv_orthogonalize: HOST arrays of device pointers g -> out [rows][cols], both dtype
  * cpcsv_muon_step: w, g, m fp32; hyper: device {lr}.  m <- momentum m + g;  U = nesterov ? g + momentum m : m;
@@ -775,6 +775,7 @@ int cpcsv_norm_residual_bwd(const void* x, const void* u, const void* gate, cons
  * The arrays are read before the call returns. No atomics: results do not depend on the run. */
 #define CPCSV_ORTH_JOBS 16
 #define CPCSV_ORTH_MAX_SIDE 131072
+#define CPCSV_ORTH_MAX_MIN 16384   /* of the shorter side */
 long cpcsv_orth_workspace(const long* dims, int njobs);
 int cpcsv_orthogonalize(const void* const* g, void* const* out, const long* dims, int njobs, int dtype, int steps, float eps, void* ws,
                         void* stream);

@@ -26,6 +26,8 @@ def test_orthogonalize_refuses():
         orthogonalize(torch.zeros(0, 4))
     with pytest.raises(ValueError, match="sides of"):
         orthogonalize(torch.zeros(1, 131073))
+    with pytest.raises(ValueError, match="sides of"):
+        orthogonalize(torch.zeros(1, 1).expand(16385, 16385))
 
 
 def test_muon_refuses():
@@ -52,10 +54,11 @@ def test_entry_points_reject_bad_arguments():
     lib = _lib.load()
     header = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "cpcsv_hip.h")).read()
     val = lambda n: int(re.search(r"#define %s (\d+)" % n, header).group(1))
-    assert (val("CPCSV_ORTH_JOBS"), val("CPCSV_ORTH_MAX_SIDE")) == (_lib.ORTH_JOBS, _lib.ORTH_MAX_SIDE)
+    assert (val("CPCSV_ORTH_JOBS"), val("CPCSV_ORTH_MAX_SIDE"), val("CPCSV_ORTH_MAX_MIN")) == (_lib.ORTH_JOBS, _lib.ORTH_MAX_SIDE, _lib.ORTH_MAX_MIN)
     dims = lambda *v: (C.c_long * len(v))(*v)
     assert lib.cpcsv_orth_workspace(dims(3, 5), 0) == -1001 and lib.cpcsv_orth_workspace(dims(3, 5), 17) == -1001
     assert lib.cpcsv_orth_workspace(dims(0, 5), 1) == -1002 and lib.cpcsv_orth_workspace(dims(3, 131073), 1) == -1002
+    assert lib.cpcsv_orth_workspace(dims(16385, 16385), 1) == -1002
     assert lib.cpcsv_orth_workspace(dims(3, 5, 300, 200), 2) > lib.cpcsv_orth_workspace(dims(300, 200), 1) > 0
     ptrs = (C.c_void_p * 1)(0x1000)
     none = (C.c_void_p * 1)(None)
