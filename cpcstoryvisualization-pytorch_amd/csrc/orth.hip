@@ -25,6 +25,7 @@
 namespace {
 typedef __attribute__((ext_vector_type(8))) _Float16 half8;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(16))) uint32_t u32x16;
 
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 // Entries are bounded by spectral norms: |X| < 1.21, |A| and |P A| < 1.45, |P| < 3.45, |Q| < 3.45^k behind k iterations. The scaled
@@ -32,7 +33,7 @@ constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr float SX = 16384.f, SA = 16384.f, SP = 8192.f;
 constexpr float SQ[4] = {0.f, SP, 4096.f, 1024.f};
 constexpr int RUN = 3;                         // iterations between two X
-constexpr int PAD = 128, MAXJ = CPCSV_ORTH_JOBS, MAXT = 2 * MAXJ, NORMB = 256;
+constexpr int PAD = 128, MAXJ = CPCSV_ORTH_JOBS, MAXT = 2 * MAXJ, NORMB = 1024;      // NORMB: most blocks of a matrix' norm
 
 struct Job {
     const void* g; float* m; void* out;       // gradient, momentum (NULL: none), weight or result
@@ -83,14 +84,47 @@ __global__ __launch_bounds__(256) void orth_norm_kernel(Jobs s) {
     const int blk = blockIdx.x - j.t_norm, nb = norm_blocks(j.rows, j.cols);
     const long n = (long)j.rows * j.cols;
     double q = 0.0;
-    for (long i = (long)blk * 256 + threadIdx.x; i < n; i += (long)nb * 256) {
-        float u = ld_g(j.g, s.dtype, i);
+    auto one = [&](float u, float& m) {
         if (j.m) {
-            const float m = __fmaf_rn(s.mu, j.m[i], u);
-            j.m[i] = m;
+            m = __fmaf_rn(s.mu, m, u);
             u = s.nesterov ? __fmaf_rn(s.mu, m, u) : m;
         }
         q += (double)u * (double)u;
+    };
+    const long step = (long)nb * 256, id = (long)blk * 256 + threadIdx.x;
+    long i = id;
+    if (((uintptr_t)j.g & 15) == 0 && ((uintptr_t)j.m & 15) == 0 && s.dtype == CPCSV_F32) {          // sixteen values a thread and turn
+        const f32x4* g4 = (const f32x4*)j.g;
+        f32x4* m4 = (f32x4*)j.m;
+        long v = id;
+        for (; v + 3 * step < n / 4; v += 4 * step) {
+            f32x4 u[4], m[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                u[k] = g4[v + k * step];
+                if (j.m) m[k] = m4[v + k * step];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { float x = m[k][e]; one(u[k][e], x); m[k][e] = x; }
+                if (j.m) m4[v + k * step] = m[k];
+            }
+        }
+        for (; v < n / 4; v += step) {
+            const f32x4 u = g4[v];
+            f32x4 m = u;
+            if (j.m) m = m4[v];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { float x = m[e]; one(u[e], x); m[e] = x; }
+            if (j.m) m4[v] = m;
+        }
+        i = n / 4 * 4 + id;
+    }
+    for (; i < n; i += step) {
+        float m = j.m ? j.m[i] : 0.f;
+        one(ld_g(j.g, s.dtype, i), m);
+        if (j.m) j.m[i] = m;
     }
     __shared__ double sh[256];
     sh[threadIdx.x] = q;
@@ -108,7 +142,9 @@ __global__ __launch_bounds__(256) void orth_split_kernel(Jobs s) {
     __shared__ double sh[256];
     const int k = job_of<&Job::t_split>(s, blockIdx.x);
     const Job& j = s.j[k];
-    sh[threadIdx.x] = threadIdx.x < norm_blocks(j.rows, j.cols) ? s.part[k * NORMB + threadIdx.x] : 0.0;
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < norm_blocks(j.rows, j.cols); i += 256) sum += s.part[k * NORMB + i];
+    sh[threadIdx.x] = sum;
     __syncthreads();
     for (int o = 128; o; o >>= 1) {
         if (threadIdx.x < o) sh[threadIdx.x] += sh[threadIdx.x + o];
@@ -157,7 +193,7 @@ struct Task {
     long slab;                 // first partial tile, in floats
     int R, C, K;
     float alpha, beta, gamma;
-    int kind, t0, tiles, S, r0;               // first block, tiles, slices of K, first block of the joining launch
+    int kind, t0, tiles, whole, S, r0;        // first block; tiles, of which `whole` in one piece, the others in S slices of K; first joining block
     int rows, cols, tall;                     // OUT: of the output
 };
 struct Launch {
@@ -169,17 +205,20 @@ struct Launch {
     float* slabs;
 };
 
-// Tiles. A wavefront's share of a tile sets what it reads from LDS for each MFMA, and LDS bandwidth is what bounds the main loop:
-// 256 x 256 with 128 x 64 a wavefront runs 1245 TFLOP/s (three MFMAs a product counted) on 4096^3 against 860 for 128 x 128 with
-// 64 x 64, which packs two blocks on a CU and fills the chip at half the tiles (1024 x 18432 x 1024: 962 against 757), and 64 x 64
-// has the shortest way through a few hundred K (512^3: 6.7 us against 13.3 and 34).
+// Tiles. A wavefront's share of a tile sets what it reads from LDS for each MFMA, and LDS bandwidth is what bounds the main loop of
+// large products: 256 x 256 with 128 x 64 a wavefront runs 1245 TFLOP/s (three MFMAs a product counted) on 4096^3 against 860 for
+// 128 x 128 with 64 x 64, which packs two blocks on a CU and fills the chip at half the tiles (1024 x 18432 x 1024: 962 against 757).
+// Small products are bound by the latency of their K steps and of what stands before and behind them: 64 x 64 tiles, whose single
+// block a wavefront keeps two accumulators (a chain of dependent MFMAs half as long) and has its entries of E loaded beforehand
+// (512^3: 6.7 us for the bare product against 13.3 and 34).
 template <int BM_, int WM_, int WN_, int BK_> struct Cfg {
-    static constexpr int BM = BM_, WM = WM_, WN = WN_, BK = BK_, WC = BM / WN, T = (BM / WM) * WC * 64, CPR = BK / 8;
+    static constexpr int BM = BM_, WM = WM_, WN = WN_, BK = BK_, WC = BM / WN, NW = (BM / WM) * WC, T = NW * 64, CPR = BK / 8;
     static constexpr int LD = BM * CPR / T;                       // 16-byte loads a thread, operand plane and stage
     static constexpr int STAGE = 4 * BM * BK;                     // halves
-    static constexpr int SW = WN < 64 ? WN : 64;                  // columns of an epilogue strip
-    static constexpr int LDS = 2 * STAGE * 2 > (T / 64) * 32 * (SW + 1) * 4 ? 2 * STAGE * 2 : (T / 64) * 32 * (SW + 1) * 4;
-    static constexpr int MA = WM / 32, MB = WN / 32, ACC = MA * MB * 16;
+    static constexpr int SW = WN < 64 ? WN : 64, NB = SW / 32;    // columns of an epilogue strip, their 32 x 32 blocks
+    static constexpr int STRIP = 32 * (SW + 1);                   // words of a strip in LDS
+    static constexpr int LDS = 2 * STAGE * 2;
+    static constexpr int MA = WM / 32, MB = WN / 32, STRIPS = MA * MB / NB;
     // chunk (16 bytes) q of LDS row r lives in slot q ^ swz(r): the rows a fragment read touches together fall into all banks. The
     // DMA writes LDS in lane order, so the permutation is on the source side.
     static __device__ __forceinline__ int swz(int r) { return CPR == 4 ? (r >> 2) & 3 : (r >> 1) & 7; }
@@ -187,6 +226,7 @@ template <int BM_, int WM_, int WN_, int BK_> struct Cfg {
 using Big = Cfg<256, 128, 64, 32>;
 using Mid = Cfg<128, 64, 64, 32>;
 using Small = Cfg<64, 32, 32, 64>;
+static_assert(Big::LDS >= Big::NW * Big::STRIP * 4 && Mid::LDS >= Mid::NW * Mid::STRIP * 4 && Small::LDS >= Small::NW * Small::STRIP * 4, "strips fit");
 
 __device__ __forceinline__ void tile_of(const Task& t, int tile, int bm, int& ti, int& tj) {
     if (t.kind == SYMM) {                        // lower triangle, row by row
@@ -201,95 +241,118 @@ __device__ __forceinline__ void tile_of(const Task& t, int tile, int bm, int& ti
     }
 }
 
-// acc of one wavefront -> D. A lane's 16 values of a 32 x 32 block: column lane % 32, rows 8 (i / 4) + 4 (lane / 32) + i % 4; they
-// pass through the wavefront's own piece of LDS, 32 rows x SW columns at a time, to leave as 16-byte pieces of rows in either
+template <int I> struct Const { static constexpr int value = I; };
+template <int N, typename F> __device__ __forceinline__ void static_for(F&& f) {
+    if constexpr (N > 0) {
+        static_for<N - 1>(f);
+        f(Const<N - 1>{});
+    }
+}
+
+__device__ __forceinline__ uint32_t entry(const Launch& s, const Task& t, int r, int c, long RC) {     // of E, hi | lo << 16
+    union { uint32_t w; _Float16 h[2]; } p;
+    const _Float16* o = s.ws + t.e + (long)r * t.C + c;
+    p.h[0] = o[0];
+    p.h[1] = o[RC];
+    return p.w;
+}
+
+// One wavefront's strip, 32 rows x SW columns from (r0, c0), -> D. A lane's 16 values of a 32 x 32 block: column lane % 32, rows
+// 8 (i / 4) + 4 (lane / 32) + i % 4; they pass through the wavefront's own piece of LDS to leave as 16-byte pieces of rows in either
 // orientation.
-template <typename C>
-__device__ __forceinline__ void finish(const Launch& s, const Task& t, int ti, int tj, const f32x16 (&acc)[C::MA][C::MB], uint32_t* lds) {
-    constexpr int SW = C::SW, LDW = SW + 1, NB = SW / 32;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 31, fk = lane >> 5;
-    uint32_t* buf = lds + wave * 32 * LDW;
+template <typename C, bool EARLY>
+__device__ __forceinline__ void finish(const Launch& s, const Task& t, int r0, int c0, const f32x16 (&acc)[C::NB], uint32_t* buf, const u32x16& early) {
+    constexpr int SW = C::SW, LDW = SW + 1, NB = C::NB;
+    const int lane = threadIdx.x & 63, fr = lane & 31, fk = lane >> 5;
+    if (r0 >= t.R || c0 >= t.C || (t.kind == SYMM && r0 + 31 < c0)) return;                // (sides are multiples of a strip's)
+    const bool diag = t.kind == SYMM && r0 < c0 + SW;                                      // the strip meets the diagonal
     const long RC = (long)t.R * t.C;
     const float lr = t.kind == OUT && s.hyper ? s.hyper[0] : 0.f;
     const float keep = 1.f - lr * s.decay, step = lr * sqrtf(fmaxf(1.f, (float)t.rows / (float)t.cols));
+    asm volatile("" ::: "memory");               // (the next strip's loads are not hoisted over this one: they would not fit the registers)
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int a = 0; a < C::MA; ++a)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int b0 = 0; b0 < C::MB; b0 += NB) {
-            const int r0 = ti * C::BM + wave / C::WC * C::WM + a * 32, c0 = tj * C::BM + wave % C::WC * C::WN + b0 * 32;
-            if (r0 >= t.R || c0 >= t.C || (t.kind == SYMM && r0 + 31 < c0)) continue;      // (sides are multiples of a strip's)
-            const bool diag = t.kind == SYMM && r0 < c0 + SW;                              // the strip meets the diagonal
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int rl = (i >> 2) * 8 + fk * 4 + (i & 3), cl = b * 32 + fr, r = r0 + rl, c = c0 + cl;
-                    float v = acc[a][b0 + b][i] * t.alpha;
-                    if (t.e >= 0) {
-                        const _Float16* o = s.ws + t.e + (long)r * t.C + c;
-                        v += ((float)o[0] + (float)o[RC]) * t.beta + (r == c ? t.gamma : 0.f);
-                    }
-                    buf[rl * LDW + cl] = t.kind == OUT ? __float_as_uint(v) : split_of(v);
-                }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            if (t.kind == OUT) {
-                // rows of the output run along the strip's columns, of a tall one's along its rows
-                const int len = t.tall ? 32 : SW, lines = t.tall ? SW : 32, per = 64 / len;
-                const int sub = lane % len;
-                for (int l = lane / len; l < lines; l += per) {
-                    const float v = __uint_as_float(t.tall ? buf[sub * LDW + l] : buf[l * LDW + sub]);
-                    const int R = (t.tall ? c0 : r0) + l, Cc = (t.tall ? r0 : c0) + sub;
-                    if (R >= t.rows || Cc >= t.cols) continue;
-                    const long at = (long)R * t.cols + Cc;
-                    if (s.hyper) ((float*)t.d)[at] = ((float*)t.d)[at] * keep - step * v;
-                    else if (s.dtype == CPCSV_F32) ((float*)t.d)[at] = v;
-                    else ((bf16_t*)t.d)[at] = f32_to_bf16(v);
-                }
-                continue;
+        for (int i = 0; i < 16; ++i) {
+            const int rl = (i >> 2) * 8 + fk * 4 + (i & 3), cl = b * 32 + fr, r = r0 + rl, c = c0 + cl;
+            float v = acc[b][i] * t.alpha;
+            if (t.e >= 0) {
+                union { uint32_t w; _Float16 h[2]; } p;
+                if (EARLY) p.w = early[i];                    // (one block a strip)
+                else p.w = entry(s, t, r, c, RC);
+                v += ((float)p.h[0] + (float)p.h[1]) * t.beta + (r == c ? t.gamma : 0.f);
             }
-            if (diag) {
-                // each pair of entries is taken from the lower one: the two sums are the same numbers in another order
-                for (int i = lane; i < 32 * SW; i += 64) {
-                    const int rl = i / SW, cl = i % SW, r = r0 + rl, c = c0 + cl;
-                    if (r < c) continue;
-                    union { uint32_t w; _Float16 h[2]; } p;
-                    p.w = buf[rl * LDW + cl];
-                    _Float16* d = s.ws + t.d;
-                    d[(long)r * t.C + c] = p.h[0];
-                    d[(long)r * t.C + c + RC] = p.h[1];
-                    d[(long)c * t.C + r] = p.h[0];
-                    d[(long)c * t.C + r + RC] = p.h[1];
-                }
-                continue;
-            }
-            uint32_t w[8];
-            half8 hi, lo;
-            constexpr int PC = SW / 8, RP = 64 / PC;              // 16-byte pieces of a strip row, rows a pass
-#pragma unroll
-            for (int i = 0; i < 32 / RP; ++i) {
-                const int rl = i * RP + lane / PC, cl = lane % PC * 8;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) w[e] = buf[rl * LDW + cl + e];
-                planes_of(w, hi, lo);
-                _Float16* d = s.ws + t.d + (long)(r0 + rl) * t.C + c0 + cl;
-                *(half8*)d = hi;
-                *(half8*)(d + RC) = lo;
-            }
-            _Float16* const turned = s.ws + (t.kind == SYMM ? t.d : t.dt);                 // (D^T [C][R]; R = C for a symmetric one)
-#pragma unroll
-            for (int i = 0; i < SW / 16; ++i) {
-                const int cl = i * 16 + lane / 4, rl = lane % 4 * 8;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) w[e] = buf[(rl + e) * LDW + cl];
-                planes_of(w, hi, lo);
-                _Float16* d = turned + (long)(c0 + cl) * t.R + r0 + rl;
-                *(half8*)d = hi;
-                *(half8*)(d + RC) = lo;
-            }
+            buf[rl * LDW + cl] = t.kind == OUT ? __float_as_uint(v) : split_of(v);
         }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    if (t.kind == OUT) {
+        // rows of the output run along the strip's columns, of a tall one's along its rows
+        const int len = t.tall ? 32 : SW, per = 64 / len, sub = lane % len;
+#pragma unroll
+        for (int i0 = 0; i0 < SW / 2; i0 += 8) {
+            float old[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int l = (i0 + i) * per + lane / len, R = (t.tall ? c0 : r0) + l, Cc = (t.tall ? r0 : c0) + sub;
+                if (s.hyper && R < t.rows && Cc < t.cols) old[i] = ((float*)t.d)[(long)R * t.cols + Cc];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int l = (i0 + i) * per + lane / len, R = (t.tall ? c0 : r0) + l, Cc = (t.tall ? r0 : c0) + sub;
+                const float v = __uint_as_float(t.tall ? buf[sub * LDW + l] : buf[l * LDW + sub]);
+                if (R >= t.rows || Cc >= t.cols) continue;
+                const long at = (long)R * t.cols + Cc;
+                if (s.hyper) ((float*)t.d)[at] = old[i] * keep - step * v;
+                else if (s.dtype == CPCSV_F32) ((float*)t.d)[at] = v;
+                else ((bf16_t*)t.d)[at] = f32_to_bf16(v);
+            }
+            asm volatile("" ::: "memory");       // (eight at a time: all of them would not fit the registers)
+        }
+        return;
+    }
+    if (diag) {
+        // each pair of entries is taken from the lower one: the two sums are the same numbers in another order
+        for (int i = lane; i < 32 * SW; i += 64) {
+            const int rl = i / SW, cl = i % SW, r = r0 + rl, c = c0 + cl;
+            if (r < c) continue;
+            union { uint32_t w; _Float16 h[2]; } p;
+            p.w = buf[rl * LDW + cl];
+            _Float16* d = s.ws + t.d;
+            d[(long)r * t.C + c] = p.h[0];
+            d[(long)r * t.C + c + RC] = p.h[1];
+            d[(long)c * t.C + r] = p.h[0];
+            d[(long)c * t.C + r + RC] = p.h[1];
+        }
+        return;
+    }
+    uint32_t w[8];
+    half8 hi, lo;
+    constexpr int PC = SW / 8, RP = 64 / PC;              // 16-byte pieces of a strip row, rows a pass
+#pragma unroll
+    for (int i = 0; i < 32 / RP; ++i) {
+        const int rl = i * RP + lane / PC, cl = lane % PC * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = buf[rl * LDW + cl + e];
+        planes_of(w, hi, lo);
+        _Float16* d = s.ws + t.d + (long)(r0 + rl) * t.C + c0 + cl;
+        *(half8*)d = hi;
+        *(half8*)(d + RC) = lo;
+    }
+    _Float16* const turned = s.ws + (t.kind == SYMM ? t.d : t.dt);                 // (D^T [C][R]; R = C for a symmetric one)
+#pragma unroll
+    for (int i = 0; i < SW / 16; ++i) {
+        const int cl = i * 16 + lane / 4, rl = lane % 4 * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = buf[(rl + e) * LDW + cl];
+        planes_of(w, hi, lo);
+        _Float16* d = turned + (long)(c0 + cl) * t.R + r0 + rl;
+        *(half8*)d = hi;
+        *(half8*)(d + RC) = lo;
+    }
 }
 
 template <typename C>
@@ -299,14 +362,16 @@ __global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
     // blocks go to the eight XCDs in turn: give each a contiguous run of tiles, whose operands its L2 then holds
     const int nb = gridDim.x, per = nb >> 3, rest = nb & 7, xcd = blockIdx.x & 7;
     const int unit = xcd * per + min(xcd, rest) + (blockIdx.x >> 3);
-    int k = 0;
-    while (k + 1 < s.n && unit >= s.t[k + 1].t0) ++k;
-    const Task& t = s.t[k];
-    const int tile = (unit - t.t0) % t.tiles, sl = (unit - t.t0) / t.tiles;
+    // (all first blocks compared at once: a search would be a chain of dependent loads)
+    const int lane = threadIdx.x & 63, first = s.t[min(lane, s.n - 1)].t0;
+    const Task& t = s.t[__popcll(__ballot(lane < s.n && unit >= first)) - 1];
+    // the whole tiles first, then the others, slice by slice
+    const int u = unit - t.t0, cut = t.tiles - t.whole;
+    const int S = u < t.whole ? 1 : t.S, sl = u < t.whole ? 0 : (u - t.whole) / cut, tile = u < t.whole ? u : t.whole + (u - t.whole) % cut;
     int ti, tj;
     tile_of(t, tile, C::BM, ti, tj);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, K = t.K;
-    const int nk = K / C::BK, k0 = (int)((long)nk * sl / t.S), k1 = (int)((long)nk * (sl + 1) / t.S);
+    const int tid = threadIdx.x, wave = tid >> 6, K = t.K;
+    const int nk = K / C::BK, k0 = (int)((long)nk * sl / S), k1 = (int)((long)nk * (sl + 1) / S);
     const _Float16* src[2] = {s.ws + t.p + (long)ti * C::BM * K, s.ws + t.q + (long)tj * C::BM * K};
     const long pl[2] = {(long)t.R * K, (long)t.C * K};
     int off[2][C::LD];                           // (K <= 131072 and 256 rows: below 2^31)
@@ -330,14 +395,24 @@ __global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
                                                                                                (i * C::T + wave * 64) * 8), 16, 0, 0);
     };
     const int wm = wave / C::WC * C::WM, wn = wave % C::WC * C::WN, fr = lane & 31, fk = lane >> 5;
-    f32x16 acc[C::MA][C::MB];
+    f32x16 acc[C::MA][C::MB], low;               // low: the hi lo terms of a one-block wavefront
 #pragma unroll
-    for (int a = 0; a < C::MA; ++a)
+    for (int e = 0; e < 16; ++e) {
+        low[e] = 0.f;
 #pragma unroll
-        for (int b = 0; b < C::MB; ++b)
+        for (int a = 0; a < C::MA; ++a)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
+            for (int b = 0; b < C::MB; ++b) acc[a][b][e] = 0.f;
+    }
     if (k0 < k1) stage(0, k0);
+    constexpr bool ONE = C::MA * C::MB == 1;
+    u32x16 early = {};
+    if (ONE && t.e >= 0 && S == 1) {
+        const int r0 = ti * C::BM + wm, c0 = tj * C::BM + wn;
+        if (r0 < t.R && c0 < t.C)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) early[i] = entry(s, t, r0 + (i >> 2) * 8 + fk * 4 + (i & 3), c0 + fr, (long)t.R * t.C);
+    }
     for (int kt = k0; kt < k1; ++kt) {
         const int buf = (kt - k0) & 1;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -360,22 +435,25 @@ __global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
                     fq[p][b] = *(const half8*)(base + (2 + p) * C::BM * C::BK + row * C::BK + ((kk * 2 + fk) ^ C::swz(row)) * 8);
                 }
             }
+#define FOR_ACC for (int a = 0; a < C::MA; ++a) _Pragma("unroll") for (int b = 0; b < C::MB; ++b)
+            if (ONE) {
+                low = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[0][0], fq[1][0], low, 0, 0, 0);
+                acc[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[0][0], fq[0][0], acc[0][0], 0, 0, 0);
+                low = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[1][0], fq[0][0], low, 0, 0, 0);
+            } else {
 #pragma unroll
-            for (int a = 0; a < C::MA; ++a)
+                FOR_ACC acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[0][a], fq[1][b], acc[a][b], 0, 0, 0);
 #pragma unroll
-                for (int b = 0; b < C::MB; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[0][a], fq[1][b], acc[a][b], 0, 0, 0);
+                FOR_ACC acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[1][a], fq[0][b], acc[a][b], 0, 0, 0);
 #pragma unroll
-            for (int a = 0; a < C::MA; ++a)
-#pragma unroll
-                for (int b = 0; b < C::MB; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[1][a], fq[0][b], acc[a][b], 0, 0, 0);
-#pragma unroll
-            for (int a = 0; a < C::MA; ++a)
-#pragma unroll
-                for (int b = 0; b < C::MB; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[0][a], fq[0][b], acc[a][b], 0, 0, 0);
+                FOR_ACC acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[0][a], fq[0][b], acc[a][b], 0, 0, 0);
+            }
         }
     }
-    if (t.S > 1) {                               // a slice's share of the tile, in the order the registers hold it
-        f32x4* d = (f32x4*)(s.slabs + t.slab) + (long)(tile * t.S + sl) * (C::ACC / 4) * C::T + tid;
+    __syncthreads();
+    if (ONE) acc[0][0] += low;
+    if (S > 1) {                                 // a slice's share of the tile, strip by strip in the order the registers hold it
+        f32x4* d = (f32x4*)(s.slabs + t.slab) + ((long)(tile - t.whole) * S + sl) * (C::BM * C::BM / 4) + (long)wave * C::STRIPS * C::NB * 256 + lane;
 #pragma unroll
         for (int a = 0; a < C::MA; ++a)
 #pragma unroll
@@ -383,76 +461,76 @@ __global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
                     f32x4 v = {acc[a][b][h * 4], acc[a][b][h * 4 + 1], acc[a][b][h * 4 + 2], acc[a][b][h * 4 + 3]};
-                    d[((a * C::MB + b) * 4 + h) * C::T] = v;
+                    d[((a * C::MB + b) * 4 + h) * 64] = v;
                 }
         return;
     }
-    __syncthreads();
-    finish<C>(s, t, ti, tj, acc, (uint32_t*)smem);
+    static_for<C::STRIPS>([&](auto i) {          // (a loop of this body is too long for the unroller, and its registers need constant indices)
+        constexpr int a = decltype(i)::value / (C::MB / C::NB), b = decltype(i)::value % (C::MB / C::NB) * C::NB;
+        f32x16 strip[C::NB];
+#pragma unroll
+        for (int n = 0; n < C::NB; ++n) strip[n] = acc[a][b + n];
+        finish<C, ONE>(s, t, ti * C::BM + wm + a * 32, tj * C::BM + wn + b * 32, strip, (uint32_t*)smem + wave * C::STRIP, early);
+    });
 }
 
-// slices of a tile, added in order
+// the slices of a tile, added in order: one wavefront a strip
 template <typename C>
-__global__ __launch_bounds__(C::T) void orth_join_kernel(Launch s) {
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    int k = 0;
-    while (k + 1 < s.n && (int)blockIdx.x >= s.t[k + 1].r0) ++k;
-    const Task& t = s.t[k];
-    const int tile = blockIdx.x - t.r0;
+__global__ __launch_bounds__(64) void orth_join_kernel(Launch s) {
+    __shared__ uint32_t buf[C::STRIP];
+    const int first = s.t[min((int)threadIdx.x, s.n - 1)].r0;
+    const Task& t = s.t[__popcll(__ballot((int)threadIdx.x < s.n && (int)blockIdx.x >= first)) - 1];
+    const int id = blockIdx.x - t.r0, strip = id % (C::NW * C::STRIPS), cut = id / (C::NW * C::STRIPS), wave = strip / C::STRIPS;
+    const int a = strip % C::STRIPS / (C::MB / C::NB), b = strip % (C::MB / C::NB) * C::NB;
     int ti, tj;
-    tile_of(t, tile, C::BM, ti, tj);
-    const f32x4* d = (const f32x4*)(s.slabs + t.slab) + (long)tile * t.S * (C::ACC / 4) * C::T + threadIdx.x;
-    f32x16 acc[C::MA][C::MB];
+    tile_of(t, t.whole + cut, C::BM, ti, tj);
+    const f32x4* d = (const f32x4*)(s.slabs + t.slab) + (long)cut * t.S * (C::BM * C::BM / 4) + (long)strip * C::NB * 256 + threadIdx.x;
+    f32x16 acc[C::NB];
 #pragma unroll
-    for (int a = 0; a < C::MA; ++a)
+    for (int n = 0; n < C::NB; ++n)
 #pragma unroll
-        for (int b = 0; b < C::MB; ++b)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
+        for (int e = 0; e < 16; ++e) acc[n][e] = 0.f;
+#pragma unroll 4
     for (int sl = 0; sl < t.S; ++sl)
 #pragma unroll
-        for (int a = 0; a < C::MA; ++a)
+        for (int n = 0; n < C::NB; ++n)
 #pragma unroll
-            for (int b = 0; b < C::MB; ++b)
+            for (int h = 0; h < 4; ++h) {
+                const f32x4 v = d[(long)sl * (C::BM * C::BM / 4) + (n * 4 + h) * 64];
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    const f32x4 v = d[((long)sl * (C::ACC / 4) + (a * C::MB + b) * 4 + h) * C::T];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[a][b][h * 4 + e] += v[e];
-                }
-    finish<C>(s, t, ti, tj, acc, (uint32_t*)smem);
+                for (int e = 0; e < 4; ++e) acc[n][h * 4 + e] += v[e];
+            }
+    finish<C, false>(s, t, ti * C::BM + wave / C::WC * C::WM + a * 32, tj * C::BM + wave % C::WC * C::WN + b * 32, acc, buf, u32x16{});
 }
 
 // ---- host: the schedule ---------------------------------------------------------------------------------------------
-// Slices of K depend on the product alone, so that a matrix has the same bits in any company: a product whose 128 x 128 tiles leave
-// CUs idle is cut into enough slices to fill them twice, none shorter than 512. (1024 x 18432 against itself: 36 tiles took 470 us.)
-int slices(int kind, long R, long C, long K) {
-    const long tm = (R + 127) / 128, tn = (C + 127) / 128, tiles = kind == SYMM ? tm * (tm + 1) / 2 : tm * tn;
-    return (int)max(1L, min((512 + tiles - 1) / tiles, K / 512 > 1 && K >= 2048 ? K / 512 : 1));
+long tiles_of(int kind, long R, long C, int bm) {
+    const long tm = (R + bm - 1) / bm, tn = (C + bm - 1) / bm;
+    return kind == SYMM ? tm * (tm + 1) / 2 : tm * tn;
 }
-long tiles_of(const Task& t, int bm) {
-    const long tm = (t.R + bm - 1) / bm, tn = (t.C + bm - 1) / bm;
-    return t.kind == SYMM ? tm * (tm + 1) / 2 : tm * tn;
-}
-// The tile of a launch: the least of (whole rounds of blocks over 256 CUs) x (K steps) x (measured time of a step), with a block's
-// fixed part. Times in us; `two`: of a step when two blocks share the CU (Big: one fits).
+// How a product is cut: the tile, and how many slices of K the tiles get that do not fill the last round of blocks over the 256 CUs
+// (all of them, where there are few: 1024 x 18432 against itself has 36 of 128 x 128 and took 470 us in one piece). By the
+// product's sides alone, so that a matrix has the same bits in any company. Least time by what a K step was measured to take (us;
+// `two`: while two blocks share the CU) and a block's fixed part; a join reads and writes its slabs once.
 struct Shape { int bm, bk, fit; double one, two, fixed; };
-constexpr Shape SHAPES[3] = {{256, 32, 1, 2.4, 2.4, 5.0}, {128, 32, 2, 0.72, 1.6, 3.0}, {64, 64, 2, 0.57, 1.14, 2.0}};
-int pick(const Launch& s) {
-    int best = 0;
+constexpr Shape SHAPES[3] = {{256, 32, 1, 2.5, 2.5, 30.0}, {128, 32, 2, 0.9, 1.6, 10.0}, {64, 64, 2, 0.57, 1.14, 4.0}};
+struct Cut { int shape, whole, S; long slab; };               // slab: floats
+Cut cut_of(int kind, long R, long C, long K) {
+    Cut best{0, 0, 1, 0};
     double least = 1e30;
     for (int c = 0; c < 3; ++c) {
-        double units = 0, steps = 0, longest = 0;
-        for (int i = 0; i < s.n; ++i) {
-            const double u = (double)tiles_of(s.t[i], SHAPES[c].bm) * s.t[i].S, n = (double)s.t[i].K / SHAPES[c].bk / s.t[i].S;
-            units += u;
-            steps += u * n;
-            longest = n > longest ? n : longest;
+        const Shape& h = SHAPES[c];
+        const long n = tiles_of(kind, R, C, h.bm), slots = 256L * h.fit, nk = K / h.bk, whole = n / slots * slots, rest = n - whole;
+        const double base = (double)(whole / slots) * (nk * h.two + h.fixed);
+        for (int S = 1; S <= 128 && (S == 1 || (rest && K / S >= 256 && rest * S <= slots)); ++S) {
+            double us = base;
+            if (rest) us += (double)((nk + S - 1) / S) * (rest * S <= 256 ? h.one : h.two) + h.fixed;
+            if (S > 1) us += 8.0 + 2.0 * rest * S * h.bm * h.bm * 4 / 4e6;
+            if (us < least) {
+                least = us;
+                best = Cut{c, (int)(S > 1 ? whole : n), S, S > 1 ? rest * S * h.bm * h.bm : 0};
+            }
         }
-        const double slots = 256.0 * SHAPES[c].fit, n = steps / units, full = (double)(long)(units / slots), rest = units - full * slots;
-        double us = full * (n * SHAPES[c].two + SHAPES[c].fixed);
-        if (rest > 0) us += (full ? n : longest) * (rest <= 256 ? SHAPES[c].one : SHAPES[c].two) + SHAPES[c].fixed;
-        if (us < least) { least = us; best = c; }
     }
     return best;
 }
@@ -462,7 +540,7 @@ struct Scratch { long a, p0, p1, r, q0, q1, xt1; };          // M x M matrices o
 
 int plan(Jobs& s, Scratch* sc, const long* dims, int njobs, Plan& p) {
     if (njobs <= 0 || njobs > MAXJ || !dims) return -1001;
-    long at = 0, slabs = 0;
+    long at = 0, gram = 0, small = 0, apply = 0;
     p = Plan{0, 0, 0, 0, 0};
     for (int i = 0; i < njobs; ++i) {
         const long r = dims[2 * i], c = dims[2 * i + 1];
@@ -481,12 +559,11 @@ int plan(Jobs& s, Scratch* sc, const long* dims, int njobs, Plan& p) {
         const long t64 = (long)(j.M / 64) * (j.N / 64);
         if (p.split + t64 > (1L << 30)) return -1002;
         p.split += (int)t64;
-        // (a tile of any shape has at most the slices' floats; sides hang over by less than a 256 tile)
-        const long need = max((long)slices(SYMM, j.M, j.M, j.N) * (j.M + 256) * (j.M + 256) * (slices(SYMM, j.M, j.M, j.N) > 1),
-                              max((long)slices(SYMM, j.M, j.M, j.M) * (j.M + 256) * (j.M + 256) * 2 * (slices(SYMM, j.M, j.M, j.M) > 1),
-                                  (long)slices(BOTH, j.M, j.N, j.M) * (j.M + 256) * (j.N + 256) * (slices(BOTH, j.M, j.N, j.M) > 1)));
-        slabs += need;
+        gram += cut_of(SYMM, j.M, j.M, j.N).slab;               // (a level holds one product of a job, two of its M x M ones)
+        small += 2 * cut_of(SYMM, j.M, j.M, j.M).slab;
+        apply += cut_of(BOTH, j.M, j.N, j.M).slab;
     }
+    const long slabs = max(gram, max(small, apply));
     s.n = njobs;
     p.planes = at;
     p.slabs = slabs;
@@ -494,42 +571,47 @@ int plan(Jobs& s, Scratch* sc, const long* dims, int njobs, Plan& p) {
     return 0;
 }
 
-template <typename C> int go(Launch& s, long slabs, hipStream_t st) {
-    int units = 0, joins = 0;
-    long at = 0;
+template <typename C> int go(Launch& s, hipStream_t st) {
+    if (!s.n) return 0;
+    long units = 0, joins = 0;
+    Launch only = s;                                            // the sliced products alone
+    only.n = 0;
     for (int i = 0; i < s.n; ++i) {
         Task& t = s.t[i];
-        const long n = tiles_of(t, C::BM);
-        t.tiles = (int)n;
-        t.t0 = units; t.r0 = joins; t.slab = at;
-        if (units + n * t.S > (1L << 30)) return -1002;
-        units += (int)(n * t.S);
+        t.t0 = (int)units; t.r0 = (int)joins;
+        units += t.whole + (long)(t.tiles - t.whole) * t.S;
         if (t.S > 1) {
-            joins += (int)n;
-            at += n * t.S * C::BM * C::BM;
+            joins += (long)(t.tiles - t.whole) * C::NW * C::STRIPS;
+            only.t[only.n++] = t;
         }
+        if (units > (1L << 30) || joins > (1L << 30)) return -1002;
     }
-    if (at > slabs) return -1004;
     if (C::LDS > 64 * 1024) {                                   // more than the default cap of dynamic LDS: raise it once
-        static const hipError_t a = hipFuncSetAttribute(reinterpret_cast<const void*>(orth_gemm_kernel<C>), hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
-        static const hipError_t b = hipFuncSetAttribute(reinterpret_cast<const void*>(orth_join_kernel<C>), hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
-        if (a != hipSuccess || b != hipSuccess) return -(int)(a != hipSuccess ? a : b);
+        static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(orth_gemm_kernel<C>), hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
+        if (e != hipSuccess) return -(int)e;
     }
-    orth_gemm_kernel<C><<<units, C::T, C::LDS, st>>>(s);
-    if (joins) {
-        Launch only = s;                                        // the sliced products alone
-        only.n = 0;
-        for (int i = 0; i < s.n; ++i)
-            if (s.t[i].S > 1) only.t[only.n++] = s.t[i];
-        orth_join_kernel<C><<<joins, C::T, (C::T / 64) * 32 * (C::SW + 1) * 4, st>>>(only);
-    }
+    orth_gemm_kernel<C><<<(int)units, C::T, C::LDS, st>>>(s);
+    if (joins) orth_join_kernel<C><<<(int)joins, 64, 0, st>>>(only);
     CPCSV_CHECK_LAUNCH();
     return 0;
 }
-int run_level(Launch& s, long slabs, hipStream_t st) {
-    if (!s.n) return 0;
-    const int c = pick(s);
-    return c == 0 ? go<Big>(s, slabs, st) : c == 1 ? go<Mid>(s, slabs, st) : go<Small>(s, slabs, st);
+// the products of one level, a launch for each tile shape among them
+int run_level(const Launch& all, long slabs, hipStream_t st) {
+    long at = 0;
+    Launch by[3];
+    for (int c = 0; c < 3; ++c) { by[c] = all; by[c].n = 0; }
+    for (int i = 0; i < all.n; ++i) {
+        Task t = all.t[i];
+        const Cut cut = cut_of(t.kind, t.R, t.C, t.K);
+        t.tiles = (int)tiles_of(t.kind, t.R, t.C, SHAPES[cut.shape].bm);
+        t.whole = cut.whole; t.S = cut.S; t.slab = at;
+        at += cut.slab;
+        by[cut.shape].t[by[cut.shape].n++] = t;
+    }
+    if (at > slabs) return -1004;
+    if (int rc = go<Big>(by[0], st)) return rc;
+    if (int rc = go<Mid>(by[1], st)) return rc;
+    return go<Small>(by[2], st);
 }
 
 int iterate(Jobs& s, const Scratch* sc, const Plan& p, int steps, const float* hyper, float decay, void* ws, hipStream_t st) {
@@ -544,7 +626,6 @@ int iterate(Jobs& s, const Scratch* sc, const Plan& p, int steps, const float* h
         Task& t = L.t[L.n++];
         t = Task{};
         t.p = pp; t.q = q; t.d = d; t.e = -1; t.R = j.M; t.C = C; t.K = K; t.alpha = alpha; t.kind = kind;
-        t.S = slices(kind, t.R, t.C, t.K);
         return t;
     };
     auto level = [&]() { const int rc = run_level(L, p.slabs, st); L.n = 0; return rc; };
