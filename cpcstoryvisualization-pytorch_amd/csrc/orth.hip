@@ -208,11 +208,12 @@ struct Launch {
 // Tiles. A wavefront's share of a tile sets what it reads from LDS for each MFMA, and LDS bandwidth is what bounds the main loop of
 // large products: 256 x 256 with 128 x 64 a wavefront runs 1245 TFLOP/s (three MFMAs a product counted) on 4096^3 against 860 for
 // 128 x 128 with 64 x 64, which packs two blocks on a CU and fills the chip at half the tiles (1024 x 18432 x 1024: 962 against 757).
-// Small products are bound by the latency of their K steps and of what stands before and behind them: 64 x 64 tiles, whose single
-// block a wavefront keeps two accumulators (a chain of dependent MFMAs half as long) and has its entries of E loaded beforehand
+// Small products are bound by the latency of their K steps and of what stands before and behind them: 64 x 64 tiles with twice the
+// wavefronts (KG = 2: each half of them takes half of a stage's K, the sums meet in LDS), whose single block a wavefront keeps two
+// accumulators (a chain of dependent MFMAs half as long) and has its entries of E loaded beforehand
 // (512^3: 6.7 us for the bare product against 13.3 and 34).
-template <int BM_, int WM_, int WN_, int BK_> struct Cfg {
-    static constexpr int BM = BM_, WM = WM_, WN = WN_, BK = BK_, WC = BM / WN, NW = (BM / WM) * WC, T = NW * 64, CPR = BK / 8;
+template <int BM_, int WM_, int WN_, int BK_, int KG_> struct Cfg {
+    static constexpr int BM = BM_, WM = WM_, WN = WN_, BK = BK_, KG = KG_, WC = BM / WN, NW = (BM / WM) * WC, T = NW * KG * 64, CPR = BK / 8;
     static constexpr int LD = BM * CPR / T;                       // 16-byte loads a thread, operand plane and stage
     static constexpr int STAGE = 4 * BM * BK;                     // halves
     static constexpr int SW = WN < 64 ? WN : 64, NB = SW / 32;    // columns of an epilogue strip, their 32 x 32 blocks
@@ -223,10 +224,11 @@ template <int BM_, int WM_, int WN_, int BK_> struct Cfg {
     // DMA writes LDS in lane order, so the permutation is on the source side.
     static __device__ __forceinline__ int swz(int r) { return CPR == 4 ? (r >> 2) & 3 : (r >> 1) & 7; }
 };
-using Big = Cfg<256, 128, 64, 32>;
-using Mid = Cfg<128, 64, 64, 32>;
-using Small = Cfg<64, 32, 32, 64>;
-static_assert(Big::LDS >= Big::NW * Big::STRIP * 4 && Mid::LDS >= Mid::NW * Mid::STRIP * 4 && Small::LDS >= Small::NW * Small::STRIP * 4, "strips fit");
+using Big = Cfg<256, 128, 64, 32, 1>;
+using Mid = Cfg<128, 64, 64, 32, 1>;
+using Small = Cfg<64, 32, 32, 64, 2>;
+static_assert(Big::LDS >= Big::NW * Big::STRIP * 4 && Mid::LDS >= Mid::NW * Mid::STRIP * 4 && Small::LDS >= Small::NW * (Small::STRIP + 1024) * 4,
+              "the epilogue's strips, and the second half of K before them, fit the stages' LDS");
 
 __device__ __forceinline__ void tile_of(const Task& t, int tile, int bm, int& ti, int& tj) {
     if (t.kind == SYMM) {                        // lower triangle, row by row
@@ -315,17 +317,32 @@ __device__ __forceinline__ void finish(const Launch& s, const Task& t, int r0, i
         return;
     }
     if (diag) {
-        // each pair of entries is taken from the lower one: the two sums are the same numbers in another order
-        for (int i = lane; i < 32 * SW; i += 64) {
-            const int rl = i / SW, cl = i % SW, r = r0 + rl, c = c0 + cl;
-            if (r < c) continue;
-            union { uint32_t w; _Float16 h[2]; } p;
-            p.w = buf[rl * LDW + cl];
-            _Float16* d = s.ws + t.d;
-            d[(long)r * t.C + c] = p.h[0];
-            d[(long)r * t.C + c + RC] = p.h[1];
-            d[(long)c * t.C + r] = p.h[0];
-            d[(long)c * t.C + r + RC] = p.h[1];
+        // by 32 x 32 blocks: below the diagonal as elsewhere; on it, each pair of entries is taken from the lower one (the two sums
+        // are the same numbers in another order)
+        uint32_t w[8];
+        half8 hi, lo;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int cb = c0 + b * 32;
+            if (cb > r0) continue;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int line = i * 16 + lane / 4, q = lane % 4 * 8;
+                const uint32_t* z = buf + b * 32;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = cb == r0 && line < q + e ? z[(q + e) * LDW + line] : z[line * LDW + q + e];
+                planes_of(w, hi, lo);
+                _Float16* d = s.ws + t.d + (long)(r0 + line) * t.C + cb + q;
+                *(half8*)d = hi;
+                *(half8*)(d + RC) = lo;
+                if (cb == r0) continue;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = z[(q + e) * LDW + line];
+                planes_of(w, hi, lo);
+                d = s.ws + t.d + (long)(cb + line) * t.C + r0 + q;
+                *(half8*)d = hi;
+                *(half8*)(d + RC) = lo;
+            }
         }
         return;
     }
@@ -359,18 +376,24 @@ template <typename C>
 __global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     _Float16* const lds = (_Float16*)smem;
-    // blocks go to the eight XCDs in turn: give each a contiguous run of tiles, whose operands its L2 then holds
-    const int nb = gridDim.x, per = nb >> 3, rest = nb & 7, xcd = blockIdx.x & 7;
-    const int unit = xcd * per + min(xcd, rest) + (blockIdx.x >> 3);
     // (all first blocks compared at once: a search would be a chain of dependent loads)
-    const int lane = threadIdx.x & 63, first = s.t[min(lane, s.n - 1)].t0;
-    const Task& t = s.t[__popcll(__ballot(lane < s.n && unit >= first)) - 1];
-    // the whole tiles first, then the others, slice by slice
-    const int u = unit - t.t0, cut = t.tiles - t.whole;
-    const int S = u < t.whole ? 1 : t.S, sl = u < t.whole ? 0 : (u - t.whole) / cut, tile = u < t.whole ? u : t.whole + (u - t.whole) % cut;
+    const int lane = threadIdx.x & 63;
+    int k = 0;
+    if (s.n > 1) {
+        const int first = s.t[min(lane, s.n - 1)].t0;
+        k = __popcll(__ballot(lane < s.n && (int)blockIdx.x >= first)) - 1;
+    }
+    const Task& t = s.t[k];
+    // the whole tiles first, then the others, slice by slice. Blocks go to the eight XCDs in turn: each gets a contiguous run of
+    // either part, whose operands its L2 then holds, and a share of both
+    const bool sliced = (int)blockIdx.x - t.t0 >= t.whole;
+    const int from = t.t0 + (sliced ? t.whole : 0), cut = t.tiles - t.whole, n = sliced ? cut * t.S : t.whole, xcd = blockIdx.x & 7;
+    int u = (blockIdx.x - from) >> 3;
+    for (int x = 0; x < xcd; ++x) u += (n + 7 - ((x - from) & 7)) >> 3;
+    const int S = sliced ? t.S : 1, sl = sliced ? u / cut : 0, tile = sliced ? t.whole + u % cut : u;
     int ti, tj;
     tile_of(t, tile, C::BM, ti, tj);
-    const int tid = threadIdx.x, wave = tid >> 6, K = t.K;
+    const int tid = threadIdx.x, wave = (tid >> 6) % C::NW, kg = (tid >> 6) / C::NW, K = t.K;
     const int nk = K / C::BK, k0 = (int)((long)nk * sl / S), k1 = (int)((long)nk * (sl + 1) / S);
     const _Float16* src[2] = {s.ws + t.p + (long)ti * C::BM * K, s.ws + t.q + (long)tj * C::BM * K};
     const long pl[2] = {(long)t.R * K, (long)t.C * K};
@@ -392,7 +415,7 @@ __global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
                 for (int i = 0; i < C::LD; ++i)
                     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[o] + (p ? pl[o] : 0) + off[o][i] + kt * C::BK),
                                                      (__attribute__((address_space(3))) void*)(lds + buf * C::STAGE + (o * 2 + p) * C::BM * C::BK +
-                                                                                               (i * C::T + wave * 64) * 8), 16, 0, 0);
+                                                                                               (i * C::T + (tid >> 6) * 64) * 8), 16, 0, 0);
     };
     const int wm = wave / C::WC * C::WM, wn = wave % C::WC * C::WN, fr = lane & 31, fk = lane >> 5;
     f32x16 acc[C::MA][C::MB], low;               // low: the hi lo terms of a one-block wavefront
@@ -407,7 +430,7 @@ __global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
     if (k0 < k1) stage(0, k0);
     constexpr bool ONE = C::MA * C::MB == 1;
     u32x16 early = {};
-    if (ONE && t.e >= 0 && S == 1) {
+    if (ONE && t.e >= 0 && S == 1 && !kg) {
         const int r0 = ti * C::BM + wm, c0 = tj * C::BM + wn;
         if (r0 < t.R && c0 < t.C)
 #pragma unroll
@@ -420,7 +443,8 @@ __global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
         if (kt + 1 < k1) stage(buf ^ 1, kt + 1);
         const _Float16* base = lds + buf * C::STAGE;
 #pragma unroll
-        for (int kk = 0; kk < C::BK / 16; ++kk) {
+        for (int k2 = 0; k2 < C::BK / 16 / C::KG; ++k2) {
+            const int kk = k2 + kg * (C::BK / 16 / C::KG);
             half8 fp[2][C::MA], fq[2][C::MB];
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
@@ -452,6 +476,23 @@ __global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
     }
     __syncthreads();
     if (ONE) acc[0][0] += low;
+    if (C::KG > 1) {                             // the halves of K meet in the first wavefronts
+        f32x4* x = (f32x4*)((uint32_t*)smem + C::NW * C::STRIP) + wave * 256 + lane;
+        if (kg)
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                f32x4 v = {acc[0][0][h * 4], acc[0][0][h * 4 + 1], acc[0][0][h * 4 + 2], acc[0][0][h * 4 + 3]};
+                x[h * 64] = v;
+            }
+        __syncthreads();
+        if (kg) return;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            const f32x4 v = x[h * 64];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[0][0][h * 4 + e] += v[e];
+        }
+    }
     if (S > 1) {                                 // a slice's share of the tile, strip by strip in the order the registers hold it
         f32x4* d = (f32x4*)(s.slabs + t.slab) + ((long)(tile - t.whole) * S + sl) * (C::BM * C::BM / 4) + (long)wave * C::STRIPS * C::NB * 256 + lane;
 #pragma unroll
@@ -513,7 +554,7 @@ long tiles_of(int kind, long R, long C, int bm) {
 // product's sides alone, so that a matrix has the same bits in any company. Least time by what a K step was measured to take (us;
 // `two`: while two blocks share the CU) and a block's fixed part; a join reads and writes its slabs once.
 struct Shape { int bm, bk, fit; double one, two, fixed; };
-constexpr Shape SHAPES[3] = {{256, 32, 1, 2.5, 2.5, 30.0}, {128, 32, 2, 0.9, 1.6, 10.0}, {64, 64, 2, 0.57, 1.14, 4.0}};
+constexpr Shape SHAPES[3] = {{256, 32, 1, 2.5, 2.5, 30.0}, {128, 32, 2, 0.9, 1.6, 10.0}, {64, 64, 2, 0.5, 1.0, 7.0}};
 struct Cut { int shape, whole, S; long slab; };               // slab: floats
 Cut cut_of(int kind, long R, long C, long K) {
     Cut best{0, 0, 1, 0};
