@@ -208,34 +208,41 @@ struct Launch {
 // Tiles. A wavefront's share of a tile sets what it reads from LDS for each MFMA, and LDS bandwidth is what bounds the main loop of
 // large products: 256 x 256 with 128 x 64 a wavefront runs 1245 TFLOP/s (three MFMAs a product counted) on 4096^3 against 860 for
 // 128 x 128 with 64 x 64, which packs two blocks on a CU and fills the chip at half the tiles (1024 x 18432 x 1024: 962 against 757).
-// Small products are bound by the latency of their K steps and of what stands before and behind them: 64 x 64 tiles with twice the
-// wavefronts (KG = 2: each half of them takes half of a stage's K, the sums meet in LDS), whose single block a wavefront keeps two
-// accumulators (a chain of dependent MFMAs half as long) and has its entries of E loaded beforehand
+// Small products are bound by the latency of their K steps and of what stands before and behind them: 64 x 64 tiles, whose single
+// block a wavefront keeps two accumulators (a chain of dependent MFMAs half as long) and has its entries of E loaded beforehand
 // (512^3: 6.7 us for the bare product against 13.3 and 34).
-template <int BM_, int WM_, int WN_, int BK_, int KG_> struct Cfg {
-    static constexpr int BM = BM_, WM = WM_, WN = WN_, BK = BK_, KG = KG_, WC = BM / WN, NW = (BM / WM) * WC, T = NW * KG * 64, CPR = BK / 8;
+template <int BM_, int WM_, int WN_, int BK_> struct Cfg {
+    static constexpr int BM = BM_, WM = WM_, WN = WN_, BK = BK_, WC = BM / WN, NW = (BM / WM) * WC, T = NW * 64, CPR = BK / 8;
     static constexpr int LD = BM * CPR / T;                       // 16-byte loads a thread, operand plane and stage
     static constexpr int STAGE = 4 * BM * BK;                     // halves
     static constexpr int SW = WN < 64 ? WN : 64, NB = SW / 32;    // columns of an epilogue strip, their 32 x 32 blocks
     static constexpr int STRIP = 32 * (SW + 1);                   // words of a strip in LDS
-    static constexpr int LDS = 2 * STAGE * 2;
+    static constexpr int LDS = 2 * STAGE * 2;                     // (rings of 3 and 4 stages were no faster, and cost the second block on a CU)
     static constexpr int MA = WM / 32, MB = WN / 32, STRIPS = MA * MB / NB;
     // chunk (16 bytes) q of LDS row r lives in slot q ^ swz(r): the rows a fragment read touches together fall into all banks. The
     // DMA writes LDS in lane order, so the permutation is on the source side.
     static __device__ __forceinline__ int swz(int r) { return CPR == 4 ? (r >> 2) & 3 : (r >> 1) & 7; }
 };
-using Big = Cfg<256, 128, 64, 32, 1>;
-using Mid = Cfg<128, 64, 64, 32, 1>;
-using Small = Cfg<64, 32, 32, 64, 2>;
-static_assert(Big::LDS >= Big::NW * Big::STRIP * 4 && Mid::LDS >= Mid::NW * Mid::STRIP * 4 && Small::LDS >= Small::NW * (Small::STRIP + 1024) * 4,
-              "the epilogue's strips, and the second half of K before them, fit the stages' LDS");
+using Big = Cfg<256, 128, 64, 32>;
+using Mid = Cfg<128, 64, 64, 32>;
+using Small = Cfg<64, 32, 32, 64>;
+static_assert(Big::LDS >= Big::NW * Big::STRIP * 4 && Mid::LDS >= Mid::NW * Mid::STRIP * 4 && Small::LDS >= Small::NW * Small::STRIP * 4, "strips fit");
 
 __device__ __forceinline__ void tile_of(const Task& t, int tile, int bm, int& ti, int& tj) {
-    if (t.kind == SYMM) {                        // lower triangle, row by row
-        ti = (int)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
-        while (ti * (ti + 1) / 2 > tile) --ti;
-        while ((ti + 1) * (ti + 2) / 2 <= tile) ++ti;
-        tj = tile - ti * (ti + 1) / 2;
+    if (t.kind == SYMM) {
+        // lower triangle by blocks of g x g tiles, a row of blocks behind the other (the last one of h tile rows; on the diagonal
+        // triangles): a run of tiles shares operand rows in L2. Row by row, every XCD read the whole operand.
+        const int n = (t.R + bm - 1) / bm, g = n >= 24 ? 8 : 4;
+        int I = 0;
+        while ((I + 1) * g < n && (I + 1) * g * ((I + 1) * g + 1) / 2 <= tile) ++I;
+        const int rem = tile - I * g * (I * g + 1) / 2, h = min(g, n - I * g), J = min(rem / (g * h), I), w = rem - J * g * h;
+        if (J < I) { ti = I * g + w / g; tj = J * g + w % g; }
+        else {
+            int r = 0, left = w;
+            while (left > r) { left -= r + 1; ++r; }
+            ti = I * g + r;
+            tj = I * g + left;
+        }
     } else {                                     // bands of 8 tile rows, so that a run of tiles shares operand rows in L2
         const int tm = (t.R + bm - 1) / bm, tn = (t.C + bm - 1) / bm, g = tile / (8 * tn), gr = min(8, tm - g * 8), w = tile - g * 8 * tn;
         ti = g * 8 + w % gr;
@@ -293,17 +300,18 @@ __device__ __forceinline__ void finish(const Launch& s, const Task& t, int r0, i
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     if (t.kind == OUT) {
         // rows of the output run along the strip's columns, of a tall one's along its rows
+        constexpr int GO = C::MA * C::MB > 4 ? 8 : SW / 2;
         const int len = t.tall ? 32 : SW, per = 64 / len, sub = lane % len;
 #pragma unroll
-        for (int i0 = 0; i0 < SW / 2; i0 += 8) {
-            float old[8];
+        for (int i0 = 0; i0 < SW / 2; i0 += GO) {
+            float old[GO];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < GO; ++i) {
                 const int l = (i0 + i) * per + lane / len, R = (t.tall ? c0 : r0) + l, Cc = (t.tall ? r0 : c0) + sub;
                 if (s.hyper && R < t.rows && Cc < t.cols) old[i] = ((float*)t.d)[(long)R * t.cols + Cc];
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < GO; ++i) {
                 const int l = (i0 + i) * per + lane / len, R = (t.tall ? c0 : r0) + l, Cc = (t.tall ? r0 : c0) + sub;
                 const float v = __uint_as_float(t.tall ? buf[sub * LDW + l] : buf[l * LDW + sub]);
                 if (R >= t.rows || Cc >= t.cols) continue;
@@ -312,7 +320,7 @@ __device__ __forceinline__ void finish(const Launch& s, const Task& t, int r0, i
                 else if (s.dtype == CPCSV_F32) ((float*)t.d)[at] = v;
                 else ((bf16_t*)t.d)[at] = f32_to_bf16(v);
             }
-            asm volatile("" ::: "memory");       // (eight at a time: all of them would not fit the registers)
+            asm volatile("" ::: "memory");       // (the big tile: eight at a time, all of them would not fit the registers)
         }
         return;
     }
@@ -393,7 +401,7 @@ __global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
     const int S = sliced ? t.S : 1, sl = sliced ? u / cut : 0, tile = sliced ? t.whole + u % cut : u;
     int ti, tj;
     tile_of(t, tile, C::BM, ti, tj);
-    const int tid = threadIdx.x, wave = (tid >> 6) % C::NW, kg = (tid >> 6) / C::NW, K = t.K;
+    const int tid = threadIdx.x, wave = tid >> 6, K = t.K;
     const int nk = K / C::BK, k0 = (int)((long)nk * sl / S), k1 = (int)((long)nk * (sl + 1) / S);
     const _Float16* src[2] = {s.ws + t.p + (long)ti * C::BM * K, s.ws + t.q + (long)tj * C::BM * K};
     const long pl[2] = {(long)t.R * K, (long)t.C * K};
@@ -415,7 +423,7 @@ __global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
                 for (int i = 0; i < C::LD; ++i)
                     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[o] + (p ? pl[o] : 0) + off[o][i] + kt * C::BK),
                                                      (__attribute__((address_space(3))) void*)(lds + buf * C::STAGE + (o * 2 + p) * C::BM * C::BK +
-                                                                                               (i * C::T + (tid >> 6) * 64) * 8), 16, 0, 0);
+                                                                                               (i * C::T + wave * 64) * 8), 16, 0, 0);
     };
     const int wm = wave / C::WC * C::WM, wn = wave % C::WC * C::WN, fr = lane & 31, fk = lane >> 5;
     f32x16 acc[C::MA][C::MB], low;               // low: the hi lo terms of a one-block wavefront
@@ -430,7 +438,7 @@ __global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
     if (k0 < k1) stage(0, k0);
     constexpr bool ONE = C::MA * C::MB == 1;
     u32x16 early = {};
-    if (ONE && t.e >= 0 && S == 1 && !kg) {
+    if (ONE && t.e >= 0 && S == 1) {
         const int r0 = ti * C::BM + wm, c0 = tj * C::BM + wn;
         if (r0 < t.R && c0 < t.C)
 #pragma unroll
@@ -443,8 +451,7 @@ __global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
         if (kt + 1 < k1) stage(buf ^ 1, kt + 1);
         const _Float16* base = lds + buf * C::STAGE;
 #pragma unroll
-        for (int k2 = 0; k2 < C::BK / 16 / C::KG; ++k2) {
-            const int kk = k2 + kg * (C::BK / 16 / C::KG);
+        for (int kk = 0; kk < C::BK / 16; ++kk) {
             half8 fp[2][C::MA], fq[2][C::MB];
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
@@ -476,23 +483,6 @@ __global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
     }
     __syncthreads();
     if (ONE) acc[0][0] += low;
-    if (C::KG > 1) {                             // the halves of K meet in the first wavefronts
-        f32x4* x = (f32x4*)((uint32_t*)smem + C::NW * C::STRIP) + wave * 256 + lane;
-        if (kg)
-#pragma unroll
-            for (int h = 0; h < 4; ++h) {
-                f32x4 v = {acc[0][0][h * 4], acc[0][0][h * 4 + 1], acc[0][0][h * 4 + 2], acc[0][0][h * 4 + 3]};
-                x[h * 64] = v;
-            }
-        __syncthreads();
-        if (kg) return;
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            const f32x4 v = x[h * 64];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[0][0][h * 4 + e] += v[e];
-        }
-    }
     if (S > 1) {                                 // a slice's share of the tile, strip by strip in the order the registers hold it
         f32x4* d = (f32x4*)(s.slabs + t.slab) + ((long)(tile - t.whole) * S + sl) * (C::BM * C::BM / 4) + (long)wave * C::STRIPS * C::NB * 256 + lane;
 #pragma unroll
@@ -554,7 +544,7 @@ long tiles_of(int kind, long R, long C, int bm) {
 // product's sides alone, so that a matrix has the same bits in any company. Least time by what a K step was measured to take (us;
 // `two`: while two blocks share the CU) and a block's fixed part; a join reads and writes its slabs once.
 struct Shape { int bm, bk, fit; double one, two, fixed; };
-constexpr Shape SHAPES[3] = {{256, 32, 1, 2.5, 2.5, 30.0}, {128, 32, 2, 0.9, 1.6, 10.0}, {64, 64, 2, 0.5, 1.0, 7.0}};
+constexpr Shape SHAPES[3] = {{256, 32, 1, 2.5, 2.5, 30.0}, {128, 32, 2, 0.9, 1.6, 10.0}, {64, 64, 2, 0.57, 1.14, 7.0}};
 struct Cut { int shape, whole, S; long slab; };               // slab: floats
 Cut cut_of(int kind, long R, long C, long K) {
     Cut best{0, 0, 1, 0};
