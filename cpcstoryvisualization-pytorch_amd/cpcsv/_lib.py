@@ -227,9 +227,10 @@ SIGNATURES = {
     "cpcsv_thin4x4s2_wgrad": [_P, _P, _P, _P, _I, _I, _I, _I, _P],
     "cpcsv_layer_update": [_P, _P],
     "cpcsv_adam_chunk": [],
-    "cpcsv_scan_chunks": [_I],
+    "cpcsv_scan_states": [_I],
+    "cpcsv_scan_workspace": [_I, _I, _I, _I],
     "cpcsv_scan_fwd": [_P, _I, _L, _L, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
-    "cpcsv_scan_bwd": [_P, _I, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
+    "cpcsv_scan_bwd": [_P, _I, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
     "cpcsv_norm_residual_fwd": [_P] * 10 + [_L, _I, _I, _I, _I, _L, _F, _P],
     "cpcsv_norm_residual_part": [_L, _I, _I, _L],
     "cpcsv_norm_residual_bwd": [_P] * 17 + [_L, _I, _I, _I, _I, _L, _P],
@@ -243,8 +244,9 @@ SIGNATURES = {
     "cpcsv_arch": [],
 }
 
-_LONG = ("cpcsv_logit_head_scratch", "cpcsv_norm_residual_part", "cpcsv_orth_workspace")        # entry points that return a count as long
+_LONG = ("cpcsv_logit_head_scratch", "cpcsv_norm_residual_part", "cpcsv_orth_workspace", "cpcsv_scan_workspace")        # entry points that return a count as long
 NORM_MAX_D = 16384         # CPCSV_NORM_MAX_D
+SCAN_MAX_T = 268435456     # CPCSV_SCAN_MAX_T
 ORTH_JOBS, ORTH_MAX_SIDE, ORTH_MAX_MIN = 16, 131072, 16384         # CPCSV_ORTH_JOBS, CPCSV_ORTH_MAX_SIDE, CPCSV_ORTH_MAX_MIN
 
 _lib = None

@@ -1377,6 +1377,8 @@ def _scan_args(p, h0, lengths, out_gate, rank):
         raise ValueError("the last dimension of p holds %d equal column blocks (%s), got %d columns"
                          % (k, "f | v | o" if out_gate else "f | v", p.shape[-1]))
     dcode(p)                                       # TypeError unless fp32 / bf16
+    if rank == 3 and p.shape[1] > L.SCAN_MAX_T:
+        raise ValueError("sequences of up to %d tokens expected, got %d" % (L.SCAN_MAX_T, p.shape[1]))
     h = p.shape[-1] // k
     if h0 is not None:
         if h0.dtype != torch.float32:
@@ -1396,7 +1398,7 @@ class GatedScanFn(Function):
     """(y, h_last) of the gated linear recurrence; see gated_scan."""
 
     @staticmethod
-    def forward(ctx, p, h0, lengths, out_gate):
+    def forward(ctx, p, h0, lengths, out_gate, keep):
         b, t, h = p.shape[0], p.shape[1], p.shape[2] // (3 if out_gate else 2)
         if p.stride(2) != 1:
             p = p.contiguous()
@@ -1409,12 +1411,10 @@ class GatedScanFn(Function):
         if b == 0 or t == 0:
             last.copy_(h0) if h0 is not None else last.zero_()
         else:
-            nc = K.scan_chunks(t)
-            sA = None
-            if nc > 1:
-                hin, sA = _empty((b, nc, h), torch.float32, dev), _empty((b, nc, h), torch.float32, dev)
-            K.scan_fwd(p, h0, lengths, y, last, hin, sA, b, t, h, out_gate)
-            _runtime.keep_forced(p, h0, lengths, hin, sA)
+            if keep and K.scan_states(t):
+                hin = _empty((b, K.scan_states(t), h), torch.float32, dev)
+            ws = K.scan_fwd(p, h0, lengths, y, last, hin, b, t, h, out_gate)
+            _runtime.keep_forced(p, h0, lengths, hin, ws)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(p, h0, lengths, hin)
         ctx.out_gate = out_gate
@@ -1426,22 +1426,19 @@ class GatedScanFn(Function):
         p, h0, lengths, hin = ctx.saved_tensors
         b, t, h = p.shape[0], p.shape[1], p.shape[2] // (3 if ctx.out_gate else 2)
         if dy is None and dlast is None:
-            return None, None, None, None
+            return (None,) * 5
         dev = p.device
         dp = _empty(p.shape, p.dtype, dev)
         dh0 = _empty((b, h), torch.float32, dev) if h0 is not None and ctx.needs_input_grad[1] else None
         if b == 0 or t == 0:
             if dh0 is not None:
                 dh0.copy_(dlast) if dlast is not None else dh0.zero_()
-            return dp, dh0, None, None
+            return dp, dh0, None, None, None
         dy = torch.zeros((b, t, h), dtype=p.dtype, device=dev) if dy is None else dy.contiguous()
         dlast = dlast.contiguous() if dlast is not None else None
-        sA = sC = None
-        if hin is not None:
-            sA, sC = _empty(hin.shape, torch.float32, dev), _empty(hin.shape, torch.float32, dev)
-        K.scan_bwd(p, h0, lengths, hin, dy, dlast, dp, dh0, sA, sC, b, t, h, ctx.out_gate)
-        _runtime.keep_forced(dy, dlast, sA, sC)
-        return dp, dh0, None, None
+        ws = K.scan_bwd(p, h0, lengths, hin, dy, dlast, dp, dh0, b, t, h, ctx.out_gate)
+        _runtime.keep_forced(dy, dlast, ws)
+        return dp, dh0, None, None, None
 
 
 def gated_scan(p, h0=None, lengths=None, out_gate=True):
@@ -1450,9 +1447,11 @@ def gated_scan(p, h0=None, lengths=None, out_gate=True):
     out_gate=False: p is [B, T, 2H] and y_t = h_t. h0 fp32 [B, H] (None: zeros). lengths int32 [B]: a sequence ends there - what stands
     behind it in p is not read, its y and gradient are zero, and its last state is the one at the end (length 0: h0).
     -> (y [B, T, H] in p's type, h_last fp32 [B, H]). Differentiable in p and h0, once. The GRU's gate convention (modules.GRUCell)
-    without W_hh: the whole sequence is three launches however long it is."""
+    without W_hh: the whole sequence is two launches however long it is (one up to 32 tokens, which then has the very bits of
+    gated_scan_step token by token)."""
     _scan_args(p, h0, lengths, out_gate, 3)
-    return GatedScanFn.apply(p, h0, lengths, bool(out_gate))
+    keep = torch.is_grad_enabled() and (p.requires_grad or (h0 is not None and h0.requires_grad))
+    return GatedScanFn.apply(p, h0, lengths, bool(out_gate), keep)
 
 
 @torch.no_grad()
@@ -1466,7 +1465,7 @@ def gated_scan_step(p, h, out_gate=True):
         p = p.contiguous()
     y = _empty((p.shape[0], hid), p.dtype, p.device)
     if p.shape[0]:
-        K.scan_fwd(p.unsqueeze(1), h, None, y, h, None, None, p.shape[0], 1, hid, out_gate)
+        K.scan_fwd(p.unsqueeze(1), h, None, y, h, None, p.shape[0], 1, hid, out_gate)
         _runtime.keep_forced(p)
     return y
 

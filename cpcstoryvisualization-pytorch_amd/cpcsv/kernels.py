@@ -604,18 +604,29 @@ def batch_prep(im_desc, im_lab, im_cont, st_desc, st_lab, td):
     return im_motion, im_content, st_motion, st_text, st_mean, chars
 
 
-def scan_chunks(T):
-    return L.load().cpcsv_scan_chunks(T)
+def scan_states(T):
+    return L.load().cpcsv_scan_states(T)
 
 
-def scan_fwd(p, h0, lengths, y, h_last, hin, sA, B, T, H, out_gate):
-    _call("cpcsv_scan_fwd", ptr(p), dcode(p), p.stride(0), p.stride(1), ptr(h0), ptr(lengths), ptr(y), ptr(h_last), ptr(hin), ptr(sA),
+def _scan_ws(B, T, H, backward, dev):
+    n = L.load().cpcsv_scan_workspace(B, T, H, backward)
+    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+
+
+def scan_fwd(p, h0, lengths, y, h_last, hin, B, T, H, out_gate):
+    """Returns the call's scratch (None for short sequences)."""
+    ws = _scan_ws(B, T, H, 0, p.device)
+    _call("cpcsv_scan_fwd", ptr(p), dcode(p), p.stride(0), p.stride(1), ptr(h0), ptr(lengths), ptr(y), ptr(h_last), ptr(hin), ptr(ws),
           B, T, H, int(out_gate), stream())
+    return ws
 
 
-def scan_bwd(p, h0, lengths, hin, dy, dh_last, dp, dh0, sA, sC, B, T, H, out_gate):
+def scan_bwd(p, h0, lengths, hin, dy, dh_last, dp, dh0, B, T, H, out_gate):
+    """Returns the call's scratch (None for short sequences)."""
+    ws = _scan_ws(B, T, H, 1, p.device)
     _call("cpcsv_scan_bwd", ptr(p), dcode(p), p.stride(0), p.stride(1), ptr(h0), ptr(lengths), ptr(hin), ptr(dy), ptr(dh_last), ptr(dp),
-          ptr(dh0), ptr(sA), ptr(sC), B, T, H, int(out_gate), stream())
+          ptr(dh0), ptr(ws), B, T, H, int(out_gate), stream())
+    return ws
 
 
 def norm_residual_fwd(x, u, gate, scale, w_post, w_next, xo, z, ru, rx, rows, D, udt, gate_mode, T, eps):

@@ -734,14 +734,17 @@ int cpcsv_thin4x4s2_wgrad(const void* dz, const void* x, float* G, float* slabs,
  *   lengths  int32 [B] on the device or NULL (all T; values are clamped to 0..T): tokens behind a sequence's end are not read, their
  *            y and dp are zero, and h_last is the state at the sequence's end
  *   y, dy    [B][T][H] dtype, contiguous; dp [B][T][3H or 2H] dtype, contiguous; dh_last, dh0 fp32 [B][H] or NULL
- *   hin, sA, sC  fp32 [B][cpcsv_scan_chunks(T)][H] workspaces, needed when that count is above 1 (else NULL): hin is filled by the
- *            forward call and read by the backward call of the same inputs, the others are scratch
- * No atomics: results do not depend on the run. */
-int cpcsv_scan_chunks(int T);
+ *   hin      fp32 [B][cpcsv_scan_states(T)][H]: filled by the forward call where it is not NULL, read by the backward call of the same
+ *            inputs; not needed where that count is 0
+ *   ws       16-byte aligned scratch of cpcsv_scan_workspace(B, T, H, 0 forward | 1 backward) bytes, contents irrelevant before and after
+ * Blocks exchange published maps through ws but apply them in one order: results do not depend on the run. T up to CPCSV_SCAN_MAX_T. */
+#define CPCSV_SCAN_MAX_T 268435456
+int cpcsv_scan_states(int T);
+long cpcsv_scan_workspace(int B, int T, int H, int backward);
 int cpcsv_scan_fwd(const void* p, int dtype, long psb, long pst, const float* h0, const int* lengths, void* y, float* h_last,
-                   float* hin, float* sA, int B, int T, int H, int out_gate, void* stream);
+                   float* hin, void* ws, int B, int T, int H, int out_gate, void* stream);
 int cpcsv_scan_bwd(const void* p, int dtype, long psb, long pst, const float* h0, const int* lengths, const float* hin, const void* dy,
-                   const float* dh_last, void* dp, float* dh0, float* sA, float* sC, int B, int T, int H, int out_gate, void* stream);
+                   const float* dh_last, void* dp, float* dh0, void* ws, int B, int T, int H, int out_gate, void* stream);
 
 /* ---- norms around a block, fused with its gate and residual scale (csrc/blocknorm.hip) --------------------------------
  * Stands beside the BatchNorm entry points: root-mean-square norms over the D values of each row, no batch statistics.

@@ -43,13 +43,20 @@ def test_gated_scan_step_refuses():
 
 def test_scan_entry_points_reject_bad_arguments():
     """The C entry points answer with an error code, without a launch: unknown type, sizes, missing workspaces."""
+    import os
+    import re
     from cpcsv import _lib
     lib = _lib.load()
-    assert [lib.cpcsv_scan_chunks(t) for t in (0, 1, 32, 33, 64, 65)] == [0, 1, 1, 2, 2, 3]
-    one = 0x1000
-    assert lib.cpcsv_scan_fwd(one, 7, 1, 1, None, None, one, None, None, None, 1, 1, 1, 1, None) == -1001
-    assert lib.cpcsv_scan_fwd(one, 0, 1, 1, None, None, one, None, None, None, 0, 1, 1, 1, None) == -1001
-    assert lib.cpcsv_scan_fwd(None, 0, 1, 1, None, None, one, None, None, None, 1, 1, 1, 1, None) == -1003
-    assert lib.cpcsv_scan_fwd(one, 0, 1, 1, None, None, one, None, None, None, 1, 64, 1, 1, None) == -1003
-    assert lib.cpcsv_scan_bwd(one, 0, 1, 1, None, None, None, one, None, one, None, None, None, 1, 64, 1, 1, None) == -1003
-    assert lib.cpcsv_scan_bwd(one, 0, 1, 1, None, None, None, None, None, one, None, None, None, 1, 1, 1, 1, None) == -1003
+    header = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "cpcsv_hip.h")).read()
+    assert int(re.search(r"#define CPCSV_SCAN_MAX_T (\d+)", header).group(1)) == _lib.SCAN_MAX_T
+    assert [lib.cpcsv_scan_states(t) for t in (0, 1, 32, 33, 48, 49, _lib.SCAN_MAX_T + 1)] == [0, 0, 0, 3, 3, 4, 0]
+    assert lib.cpcsv_scan_workspace(2, 32, 8, 0) == 0 and lib.cpcsv_scan_workspace(0, 64, 8, 0) == 0
+    for back in (0, 1):
+        n = lib.cpcsv_scan_workspace(2, 5000, 9, back)
+        assert n > 2 * 9 * 8 * 5000 // 128 and n % 16 == 0
+    one, odd = 0x1000, 0x1008
+    fwd = lambda p=one, dt=0, y=one, ws=None, B=1, T=1: lib.cpcsv_scan_fwd(p, dt, 1, 1, None, None, y, None, None, ws, B, T, 1, 1, None)
+    assert fwd(dt=7) == -1001 and fwd(B=0) == -1001 and fwd(T=0) == -1001 and fwd(T=_lib.SCAN_MAX_T + 1) == -1001
+    assert fwd(p=None) == -1003 and fwd(y=None) == -1003 and fwd(T=64) == -1003 and fwd(T=64, ws=odd) == -1003
+    bwd = lambda hin=one, dy=one, dp=one, ws=one, T=64: lib.cpcsv_scan_bwd(one, 0, 1, 1, None, None, hin, dy, None, dp, None, ws, 1, T, 1, 1, None)
+    assert bwd(hin=None) == -1003 and bwd(ws=None) == -1003 and bwd(ws=odd) == -1003 and bwd(dy=None) == -1003 and bwd(dp=None, T=1) == -1003
