@@ -1370,21 +1370,21 @@ class GruSeqFn(Function):
 # ------------------------------------------------------------------------------------------------
 def _scan_args(p, h0, lengths, out_gate, rank):
     """Checks of gated_scan / gated_scan_step -> H."""
-    k = 3 if out_gate else 2
-    if p.dim() != rank:
-        raise ValueError("p must have %d dimensions, got shape %s" % (rank, tuple(p.shape)))
-    if p.shape[-1] % k or (p.shape[-1] == 0):
+    k, shape = 3 if out_gate else 2, p.shape
+    if len(shape) != rank:
+        raise ValueError("p must have %d dimensions, got shape %s" % (rank, tuple(shape)))
+    h = shape[-1] // k
+    if h * k != shape[-1] or h == 0:
         raise ValueError("the last dimension of p holds %d equal column blocks (%s), got %d columns"
-                         % (k, "f | v | o" if out_gate else "f | v", p.shape[-1]))
+                         % (k, "f | v | o" if out_gate else "f | v", shape[-1]))
     dcode(p)                                       # TypeError unless fp32 / bf16
-    if rank == 3 and p.shape[1] > L.SCAN_MAX_T:
-        raise ValueError("sequences of up to %d tokens expected, got %d" % (L.SCAN_MAX_T, p.shape[1]))
-    h = p.shape[-1] // k
+    if rank == 3 and shape[1] > L.SCAN_MAX_T:
+        raise ValueError("sequences of up to %d tokens expected, got %d" % (L.SCAN_MAX_T, shape[1]))
     if h0 is not None:
         if h0.dtype != torch.float32:
             raise TypeError("the state is held in float32, got %s" % h0.dtype)
-        if tuple(h0.shape) != (p.shape[0], h):
-            raise ValueError("the state must have shape %s, got %s" % ((p.shape[0], h), tuple(h0.shape)))
+        if h0.shape != (shape[0], h):
+            raise ValueError("the state must have shape %s, got %s" % ((shape[0], h), tuple(h0.shape)))
     if lengths is not None:
         if lengths.dtype != torch.int32:
             raise TypeError("lengths must be int32, got %s" % lengths.dtype)
@@ -1454,18 +1454,18 @@ def gated_scan(p, h0=None, lengths=None, out_gate=True):
     return GatedScanFn.apply(p, h0, lengths, bool(out_gate), keep)
 
 
-@torch.no_grad()
 def gated_scan_step(p, h, out_gate=True):
     """One token of gated_scan for every row: p [B, 3H] (2H without the output gate), h fp32 [B, H] contiguous, UPDATED IN PLACE.
-    -> y [B, H] in p's type. One launch, nothing allocated but y; for generation (no gradients)."""
+    -> y [B, H] in p's type. One launch, nothing allocated but y; for generation: no gradients (a state that requires some is refused)."""
     hid = _scan_args(p, h, None, out_gate, 2)
-    if h is None or not h.is_contiguous():
-        raise ValueError("the state is updated in place: it must be a contiguous tensor")
+    if h is None or not h.is_contiguous() or h.requires_grad:
+        raise ValueError("the state is updated in place: it must be a contiguous tensor that requires no gradient")
     if p.stride(1) != 1:
-        p = p.contiguous()
-    y = _empty((p.shape[0], hid), p.dtype, p.device)
-    if p.shape[0]:
-        K.scan_fwd(p.unsqueeze(1), h, None, y, h, None, p.shape[0], 1, hid, out_gate)
+        p = p.detach().contiguous()
+    b = p.shape[0]
+    y = _empty((b, hid), p.dtype, p.device)
+    if b:
+        K.scan_step(p, h, y, b, hid, out_gate)
         _runtime.keep_forced(p)
     return y
 

@@ -621,6 +621,12 @@ def scan_fwd(p, h0, lengths, y, h_last, hin, B, T, H, out_gate):
     return ws
 
 
+def scan_step(p, h, y, B, H, out_gate):
+    """One token: p [B][3H or 2H], h in and out."""
+    _call("cpcsv_scan_fwd", p.data_ptr(), dcode(p), p.stride(0), 0, h.data_ptr(), None, y.data_ptr(), h.data_ptr(), None, None,
+          B, 1, H, int(out_gate), stream())
+
+
 def scan_bwd(p, h0, lengths, hin, dy, dh_last, dp, dh0, B, T, H, out_gate):
     """Returns the call's scratch (None for short sequences)."""
     ws = _scan_ws(B, T, H, 1, p.device)

@@ -21,8 +21,9 @@
 
 namespace {
 constexpr int CH = 16;               // tokens a wavefront holds
-constexpr int FW = 8, BW = 6;        // wavefronts (chunks) of a tile, forward and backward: what fits the registers twice on a CU
-constexpr int SB = 16;               // tiles between published states
+constexpr int FW = 8, BW = 4;        // wavefronts (chunks) of a tile, forward and backward: what the registers hold twice on a CU
+constexpr int SB = 8;                // tiles between published states (training batch of 8 x 4096 x 2048, both directions: 16 tiles 341 us,
+                                     // 8 322, 4 315; but a state has to pass T / (SB tiles) hands, and fewer of them is safer for long T)
 constexpr int SHORT = 32;
 constexpr int TB = 256;
 constexpr int POLLS = 1 << 20;       // of a wait (about a second): a bound that no run comes near
@@ -328,7 +329,7 @@ __global__ __launch_bounds__(FW * 64, 4) void scan_fwd_kernel(const T* __restric
 // h of the chunk is run again from its entering state; what does not wait for D leaves at once (do), the rest is kept as
 // u = dy silu(o), z, 1 - z and z (1 - z) (h_{t-1} - v). Tiles and wavefronts count from the sequence's end.
 template <typename T, int VEC, bool GATE>
-__global__ __launch_bounds__(BW * 64, 3) void scan_bwd_kernel(const T* __restrict__ p, const float* __restrict__ hin, const T* __restrict__ dy,
+__global__ __launch_bounds__(BW * 64, 2) void scan_bwd_kernel(const T* __restrict__ p, const float* __restrict__ hin, const T* __restrict__ dy,
                                                               const float* __restrict__ dh_last, T* __restrict__ dp, float* __restrict__ dh0, Look lk, Dims d) {
     constexpr int K = GATE ? 3 : 2;
     __shared__ Joint<BW, VEC> sh;

@@ -276,6 +276,21 @@ def test_side_stream():
         assert torch.equal(got[k], want[k]), k
 
 
+def test_step_refuses_states_it_cannot_update():
+    from cpcsv import functional as F
+    p = torch.zeros(2, 12).cuda()
+    for h in (None, torch.zeros(4, 2).cuda().T, torch.zeros(2, 4).cuda().requires_grad_()):
+        with pytest.raises(ValueError, match="in place"):
+            F.gated_scan_step(p, h)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b,t,h,lengths", [(1, 5000, 70, None), (2, 2305, 130, [2305, 1100]), (300, 40, 6, None), (1, 129, 2000, None)])
+def test_many_tiles(b, t, h, lengths, dtype):
+    """Several published states on the way, more blocks than the chip holds, a last tile of one token."""
+    check(*make(b, t, h, True, dtype, seed=t, lengths=lengths), True)
+
+
 def test_empty():
     from cpcsv import functional as F
     h0 = torch.randn(2, 3).cuda().requires_grad_()

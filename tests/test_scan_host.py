@@ -39,6 +39,7 @@ def test_gated_scan_step_refuses():
         F.gated_scan_step(p.view(2, 1, 12), h)
     with pytest.raises(ValueError, match="state must have shape"):
         F.gated_scan_step(p, torch.zeros(2, 6))
+    assert F.L.SCAN_MAX_T == 1 << 28
 
 
 def test_scan_entry_points_reject_bad_arguments():
