@@ -6,9 +6,10 @@
 //     dgate = dx scale w_post uh    dw_next = sum dz xh    dw_post = scale sum(dx gate uh)    dscale = w_post sum(dx gate uh)
 // HBM-bound: every tensor is read or written once. x' is formed again in the backward pass from x and u (the same bytes as reading
 // it, and exactly the forward's fp32 value rather than its rounded copy), the row statistics are two floats a row.
-// A row is owned by `tpr` threads (64: one wavefront, no barrier; up to 512 for wide rows) that keep it in registers between the
-// two reductions, with their share of the weights beside it: blocks walk many rows, so the weights are read once a block. The
-// weight gradients' column sums accumulate in registers over a block's rows and are joined by a second launch in a fixed order.
+// A row is owned by `tpr` threads (64: one wavefront, no barrier; up to 1024 for wide rows) that keep 8 values each in registers
+// between the two reductions, with their share of the weights beside them: blocks walk many rows, so the weights are read once a
+// block, and the next row is loaded before this one's reductions. The weight gradients' column sums accumulate in registers over a
+// block's rows and are joined by a second launch in a fixed order.
 #include "common.h"
 #include "../../include/cpcsv_hip.h"
 
@@ -17,11 +18,26 @@ constexpr int MAXB = 1024;         // blocks of the backward kernel (and partial
 
 template <typename T, int VEC> struct alignas(sizeof(T) * VEC < 16 ? sizeof(T) * VEC : 16) word { T d[VEC]; };
 template <typename T, int VEC> __device__ __forceinline__ word<T, VEC> ldw(const T* p) { return *reinterpret_cast<const word<T, VEC>*>(p); }
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+template <typename T, int VEC> __device__ __forceinline__ void stw(T* p, const float* v) {
+    word<T, VEC> w;
+    if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {            // (one conversion of two values, rounded to nearest even)
+#pragma unroll
+        for (int k = 0; k < VEC; k += 2) {
+            const bf16x2 r = __builtin_convertvector((f32x2{v[k], v[k + 1]}), bf16x2);
+            __builtin_memcpy(&w.d[k], &r, 4);
+        }
+    } else
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) elem<T>::st(&w.d[k], v[k]);
+    *reinterpret_cast<word<T, VEC>*>(p) = w;
+}
 
 struct NormArgs {
     const void *x, *u, *gate; const float *scale, *w_post, *w_next;
     void *xo, *z; float *ru, *rx;
-    const void *dxo, *dz; void *dx, *du, *dgate; float *partE, *partF;
+    const void *dxo, *dz; void *dx, *du, *dgate; float *partE, *partF, *partE0;
     long rows, T; int D, gmode, tpr, S, items; float eps;
 };
 
@@ -32,7 +48,7 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 // sum over the row's threads, the same value (and bits) in all of them. `slot` alternates so that one barrier a reduction suffices:
 // a slot is written again only behind the barrier of the reduction in between.
-__device__ __forceinline__ float row_sum(float v, int tpr, float (*red)[8], int& slot) {
+__device__ __forceinline__ float row_sum(float v, int tpr, float (*red)[16], int& slot) {
     v = wave_sum(v);
     if (tpr == 64) return v;
     const int nw = tpr >> 6;
@@ -44,8 +60,8 @@ __device__ __forceinline__ float row_sum(float v, int tpr, float (*red)[8], int&
     return v;
 }
 
-template <int VEC, int NV> struct Cols {
-    float s[NV * VEC], wp[NV * VEC], wn[NV * VEC];
+template <int VEC, int NV> struct Cols {            // f = scale w_post
+    float f[NV * VEC], wn[NV * VEC];
     __device__ __forceinline__ void load(const NormArgs& a, int lr) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -53,8 +69,7 @@ template <int VEC, int NV> struct Cols {
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
                 const bool in = c < a.D;
-                s[j * VEC + k] = in && a.scale ? a.scale[c + k] : 1.f;
-                wp[j * VEC + k] = in && a.w_post ? a.w_post[c + k] : 0.f;
+                f[j * VEC + k] = in && a.w_post ? __fmul_rn(a.scale ? a.scale[c + k] : 1.f, a.w_post[c + k]) : 0.f;
                 wn[j * VEC + k] = in && a.w_next ? a.w_next[c + k] : 0.f;
             }
         }
@@ -65,62 +80,82 @@ template <typename T, int VEC, int NV> struct Row {
     __device__ __forceinline__ void load(const void* p, long off, const NormArgs& a, int lr, bool on) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int c = (j * a.tpr + lr) * VEC;
-            if (on && c < a.D) r[j] = ldw<T, VEC>((const T*)p + off + c);
+            const unsigned c = (j * a.tpr + lr) * VEC;
+            if (on && c < (unsigned)a.D) r[j] = ldw<T, VEC>((const T*)p + off + c);
             else
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) elem<T>::st(&r[j].d[k], 0.f);
         }
     }
     __device__ __forceinline__ float at(int i) const { return elem<T>::ld(&r[i / VEC].d[i % VEC]); }
+    // what was unpacked so far is not kept: unpacking 16-bit values again costs an instruction, holding them unpacked a register each
+    __device__ __forceinline__ void forget() {
+        if constexpr (sizeof(T) == 2 && VEC == 8)
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                u32x4 w;
+                __builtin_memcpy(&w, &r[j], 16);
+                asm volatile("" : "+v"(w));
+                __builtin_memcpy(&r[j], &w, 16);
+            }
+    }
 };
 template <typename T, int VEC, int NV>
 __device__ __forceinline__ void store_row(void* p, long off, const float* v, const NormArgs& a, int lr, bool on) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int c = (j * a.tpr + lr) * VEC;
-        if (on && c < a.D) {
-            word<T, VEC> w;
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) elem<T>::st(&w.d[k], v[j * VEC + k]);
-            *reinterpret_cast<word<T, VEC>*>((T*)p + off + c) = w;
-        }
+        const unsigned c = (j * a.tpr + lr) * VEC;
+        if (on && c < (unsigned)a.D) stw<T, VEC>((T*)p + off + c, v + j * VEC);
     }
 }
 __device__ __forceinline__ long gate_off(const NormArgs& a, long row) { return (a.gmode == 2 ? row / a.T : row) * a.D; }
 // the residual sum, its roundings pinned: forward and backward form the same x'
-__device__ __forceinline__ float residual(float x, float s, float g, float wp, float uh) { return __fmaf_rn(__fmul_rn(__fmul_rn(s, g), wp), uh, x); }
+__device__ __forceinline__ float residual(float x, float g, float f, float uh) { return __fmaf_rn(__fmul_rn(g, f), uh, x); }
+
+template <typename XT, typename UT, int VEC, int NV> struct FwdRows {
+    Row<XT, VEC, NV> x;
+    Row<UT, VEC, NV> u, g;
+    __device__ __forceinline__ void load(const NormArgs& a, long row, long end, int lr) {
+        const bool on = row < end;
+        const long off = on ? row * a.D : 0;
+        x.load(a.x, off, a, lr, on);
+        if (a.u) u.load(a.u, off, a, lr, on);
+        if (a.gmode) g.load(a.gate, on ? gate_off(a, row) : 0, a, lr, on);
+    }
+};
 
 template <typename XT, typename UT, int VEC, int NV>
-__global__ __launch_bounds__(512) void norm_fwd_kernel(NormArgs a) {
-    __shared__ float red[2][8];
+__global__ __launch_bounds__(1024) void norm_fwd_kernel(NormArgs a) {
+    __shared__ float red[2][16];
     constexpr int E = NV * VEC;
-    const int lr = threadIdx.x % a.tpr, rid = threadIdx.x / a.tpr, rpb = blockDim.x / a.tpr;
+    // (a wavefront lies in one row: its address arithmetic is scalar)
+    const int lr = threadIdx.x % a.tpr, rid = __builtin_amdgcn_readfirstlane(threadIdx.x / a.tpr), rpb = blockDim.x / a.tpr;
     const float inv = 1.f / (float)a.D;
+    const long step = (long)gridDim.x * rpb;
     int slot = 0;
+    constexpr bool AHEAD = E == 8 && VEC == 8;                  // (elsewhere two rows would not fit the registers)
+    FwdRows<XT, UT, VEC, NV> cur, next;
+    if (AHEAD) cur.load(a, (long)blockIdx.x * rpb + rid, a.rows, lr);
     Cols<VEC, NV> w;
     w.load(a, lr);
-    for (long row0 = (long)blockIdx.x * rpb; row0 < a.rows; row0 += (long)gridDim.x * rpb) {
+    for (long row0 = (long)blockIdx.x * rpb; row0 < a.rows; row0 += step) {
         const long row = row0 + rid;
         const bool on = row < a.rows;
-        Row<XT, VEC, NV> x;
-        Row<UT, VEC, NV> u, g;
-        x.load(a.x, row * a.D, a, lr, on);
+        if (!AHEAD) cur.load(a, row, a.rows, lr);
+        else if (row0 + step < a.rows) next.load(a, row + step, a.rows, lr);
         float x1[E];
         if (a.u) {
-            u.load(a.u, row * a.D, a, lr, on);
-            if (a.gmode) g.load(a.gate, on ? gate_off(a, row) : 0, a, lr, on);
             float q = 0.f;
 #pragma unroll
-            for (int i = 0; i < E; ++i) q = __fmaf_rn(u.at(i), u.at(i), q);
+            for (int i = 0; i < E; ++i) q = __fmaf_rn(cur.u.at(i), cur.u.at(i), q);
             const float ru = rsqrtf(row_sum(q, a.tpr, red, slot) * inv + a.eps);
 #pragma unroll
-            for (int i = 0; i < E; ++i) x1[i] = residual(x.at(i), w.s[i], a.gmode ? g.at(i) : 1.f, w.wp[i], __fmul_rn(u.at(i), ru));
+            for (int i = 0; i < E; ++i) x1[i] = residual(cur.x.at(i), a.gmode ? cur.g.at(i) : 1.f, w.f[i], __fmul_rn(cur.u.at(i), ru));
             store_row<XT, VEC, NV>(a.xo, row * a.D, x1, a, lr, on);
             if (on && lr == 0) a.ru[row] = ru;
         } else {
 #pragma unroll
-            for (int i = 0; i < E; ++i) x1[i] = x.at(i);
+            for (int i = 0; i < E; ++i) x1[i] = cur.x.at(i);
         }
         if (a.w_next) {
             float q = 0.f;
@@ -132,17 +167,36 @@ __global__ __launch_bounds__(512) void norm_fwd_kernel(NormArgs a) {
             store_row<UT, VEC, NV>(a.z, row * a.D, x1, a, lr, on);
             if (on && lr == 0) a.rx[row] = rx;
         }
+        if (AHEAD) cur = next;
     }
 }
+
+template <typename XT, typename UT, int VEC, int NV> struct BwdRows {
+    Row<XT, VEC, NV> x, dxo;
+    Row<UT, VEC, NV> u, g, dz;
+    float ru, rx;
+    __device__ __forceinline__ void load(const NormArgs& a, long row, long end, int lr) {
+        const bool on = row < end;
+        const long off = on ? row * a.D : 0;
+        x.load(a.x, off, a, lr, on);
+        if (a.dxo) dxo.load(a.dxo, off, a, lr, on);
+        if (a.dz) dz.load(a.dz, off, a, lr, on);
+        if (a.u) u.load(a.u, off, a, lr, on);
+        if (a.gmode) g.load(a.gate, on ? gate_off(a, row) : 0, a, lr, on);
+        ru = on && a.u ? a.ru[row] : 0.f;
+        rx = on && a.dz ? a.rx[row] : 0.f;
+    }
+};
 
 // items: with a gate a sample, (sample, segment) pairs of consecutive rows - E is kept apart for each; otherwise one item a block,
 // its rows a grid apart
 template <typename XT, typename UT, int VEC, int NV>
-__global__ __launch_bounds__(512) void norm_bwd_kernel(NormArgs a) {
-    __shared__ float red[2][8];
+__global__ __launch_bounds__(1024) void norm_bwd_kernel(NormArgs a) {
+    __shared__ float red[2][16];
     __shared__ float fold[NV * VEC == 8 ? 64 * 4 * 8 : 1];      // (several rows a block only at 8 values a thread)
     constexpr int E = NV * VEC;
-    const int lr = threadIdx.x % a.tpr, rid = threadIdx.x / a.tpr, rpb = blockDim.x / a.tpr;
+    // (a wavefront lies in one row: its address arithmetic is scalar)
+    const int lr = threadIdx.x % a.tpr, rid = __builtin_amdgcn_readfirstlane(threadIdx.x / a.tpr), rpb = blockDim.x / a.tpr;
     const float inv = 1.f / (float)a.D;
     int slot = 0;
     Cols<VEC, NV> w;
@@ -183,104 +237,101 @@ __global__ __launch_bounds__(512) void norm_bwd_kernel(NormArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < E; ++i) accE[i] = 0.f;
+        constexpr bool AHEAD = E == 8 && VEC == 8;
+        BwdRows<XT, UT, VEC, NV> cur, next;
+        if (AHEAD) cur.load(a, lo + rid, hi, lr);
         for (long row0 = lo; row0 < hi; row0 += step) {
             const long row = row0 + rid;
             const bool on = row < hi;
-            Row<XT, VEC, NV> x, dxo;
-            Row<UT, VEC, NV> u, g, dz;
-            float x1[E], uh[E], dx[E], ru = 0.f;
-            x.load(a.x, row * a.D, a, lr, on);
-            if (a.dxo) dxo.load(a.dxo, row * a.D, a, lr, on);
-            if (a.dz) dz.load(a.dz, row * a.D, a, lr, on);
-            if (a.u) {
-                u.load(a.u, row * a.D, a, lr, on);
-                if (a.gmode) g.load(a.gate, on ? gate_off(a, row) : 0, a, lr, on);
-                ru = on ? a.ru[row] : 0.f;
-            }
+            if (!AHEAD) cur.load(a, row, hi, lr);
+            else if (row0 + step < hi) next.load(a, row + step, hi, lr);
+            float xh[E], dx[E];
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                x1[i] = x.at(i);
-                if (a.u) {
-                    uh[i] = __fmul_rn(u.at(i), ru);
-                    x1[i] = residual(x1[i], w.s[i], a.gmode ? g.at(i) : 1.f, w.wp[i], uh[i]);
-                }
-                dx[i] = a.dxo ? dxo.at(i) : 0.f;
+                xh[i] = cur.x.at(i);
+                if (a.u) xh[i] = residual(xh[i], a.gmode ? cur.g.at(i) : 1.f, w.f[i], __fmul_rn(cur.u.at(i), cur.ru));
+                dx[i] = a.dxo ? cur.dxo.at(i) : 0.f;
             }
             if (a.dz) {
-                const float rx = on ? a.rx[row] : 0.f;
                 float q = 0.f;
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
-                    x1[i] *= rx;
-                    q += dz.at(i) * w.wn[i] * x1[i];
-                    accF[i] += dz.at(i) * x1[i];
+                    xh[i] *= cur.rx;
+                    q += cur.dz.at(i) * w.wn[i] * xh[i];
+                    accF[i] += cur.dz.at(i) * xh[i];
                 }
+                cur.dz.forget();
                 q = row_sum(q, a.tpr, red, slot) * inv;
 #pragma unroll
-                for (int i = 0; i < E; ++i) dx[i] += rx * (dz.at(i) * w.wn[i] - x1[i] * q);
+                for (int i = 0; i < E; ++i) dx[i] += cur.rx * (cur.dz.at(i) * w.wn[i] - xh[i] * q);
             }
             store_row<XT, VEC, NV>(a.dx, row * a.D, dx, a, lr, on);
+            cur.u.forget();
+            cur.g.forget();
             if (a.u) {
                 float q = 0.f;
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
-                    const float gt = a.gmode ? g.at(i) : 1.f, t = dx[i] * uh[i];
+                    const float gt = a.gmode ? cur.g.at(i) : 1.f, uh = __fmul_rn(cur.u.at(i), cur.ru), t = dx[i] * uh;
                     accE[i] += a.gmode == 1 ? t * gt : t;
-                    x1[i] = t * w.s[i] * w.wp[i];                          // (x1: the gate's gradient from here)
-                    dx[i] *= w.s[i] * gt * w.wp[i];
-                    q += dx[i] * uh[i];
+                    xh[i] = t * w.f[i];                                    // (the gate's gradient from here)
+                    dx[i] *= gt * w.f[i];
+                    q += dx[i] * uh;
                 }
-                if (a.gmode == 1 && a.dgate) store_row<UT, VEC, NV>(a.dgate, row * a.D, x1, a, lr, on);
+                if (a.gmode == 1 && a.dgate) store_row<UT, VEC, NV>(a.dgate, row * a.D, xh, a, lr, on);
+                cur.u.forget();
                 q = row_sum(q, a.tpr, red, slot) * inv;
 #pragma unroll
-                for (int i = 0; i < E; ++i) dx[i] = ru * (dx[i] - uh[i] * q);
+                for (int i = 0; i < E; ++i) dx[i] = cur.ru * (dx[i] - __fmul_rn(cur.u.at(i), cur.ru) * q);
                 if (a.du) store_row<UT, VEC, NV>(a.du, row * a.D, dx, a, lr, on);
             }
+            if (AHEAD) cur = next;
         }
         if (a.partE) flush(accE, a.partE + (long)item * a.D);
     }
     if (a.partF) flush(accF, a.partF + (long)blockIdx.x * a.D);
 }
 
-// a gate a sample: E of the sample's segments -> its gradient; the first segment's row becomes gate * E for the sums over samples
-template <typename UT>
-__global__ __launch_bounds__(256) void norm_gate_kernel(const UT* gate, const float* scale, const float* w_post, float* partE, UT* dgate, int B, int S, int D) {
-    const long id = (long)blockIdx.x * 256 + threadIdx.x;
-    if (id >= (long)B * D) return;
-    const long b = id / D;
-    const int c = (int)(id - b * D);
-    float e = 0.f;
-    for (int s = 0; s < S; ++s) e += partE[(b * S + s) * D + c];
-    if (dgate) elem<UT>::st(dgate + id, e * (scale ? scale[c] : 1.f) * w_post[c]);
-    partE[b * S * D + c] = e * elem<UT>::ld(gate + id);
+// 16 columns x 64 row lanes a block: the sum of n rows of `part` ld values apart, from column c; in the first row lane
+__device__ __forceinline__ float column_sum(const float* part, int n, long ld, int c, int D, float (*sh)[17]) {
+    const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4;
+    float v = 0.f;
+    if (c < D)
+        for (int r = rl; r < n; r += 64) v += part[r * ld + c];
+    sh[rl][cl] = v;
+    __syncthreads();
+    v = 0.f;
+    if (rl == 0)
+#pragma unroll
+        for (int r = 0; r < 64; ++r) v += sh[r][cl];
+    return v;
 }
 
-// column sums of the partial rows (nE of them strideE rows apart; nF): 32 columns x 32 row lanes a block
+// a gate a sample: E of the sample's segments -> its gradient; the first segment's row becomes gate * E for the sums over samples
+template <typename UT>
+__global__ __launch_bounds__(1024) void norm_gate_kernel(const UT* gate, const float* scale, const float* w_post, float* partE, UT* dgate, int S, int D) {
+    __shared__ float sh[64][17];
+    const int c = blockIdx.x * 16 + (threadIdx.x & 15);
+    const long b = blockIdx.y;
+    const float e = column_sum(partE + b * S * D, S, D, c, D, sh);
+    if (threadIdx.x >= 16 || c >= D) return;
+    if (dgate) elem<UT>::st(dgate + b * D + c, e * __fmul_rn(scale ? scale[c] : 1.f, w_post[c]));
+    partE[b * S * D + c] = e * elem<UT>::ld(gate + b * D + c);
+}
+
+// column sums of the partial rows (nE of them strideE rows apart; nF)
 __global__ __launch_bounds__(1024) void norm_cols_kernel(const float* partE, int nE, int strideE, const float* partF, int nF, const float* scale,
                                                          const float* w_post, float* dscale, float* dw_post, float* dw_next, int D) {
-    __shared__ float sh[32][33];
-    const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
-    for (int which = 0; which < 2; ++which) {
-        const float* part = which ? partF : partE;
-        if (!part) continue;
-        const int n = which ? nF : nE;
-        const long ld = (long)(which ? 1 : strideE) * D;
-        float v = 0.f;
-        if (c < D)
-            for (int r = rl; r < n; r += 32) v += part[r * ld + c];
-        __syncthreads();
-        sh[rl][cl] = v;
-        __syncthreads();
-        if (rl == 0 && c < D) {
-            v = 0.f;
-#pragma unroll
-            for (int r = 0; r < 32; ++r) v += sh[r][cl];
-            if (which) { if (dw_next) dw_next[c] = v; }
-            else {
-                if (dw_post) dw_post[c] = v * (scale ? scale[c] : 1.f);
-                if (dscale) dscale[c] = v * w_post[c];
-            }
-        }
+    __shared__ float sh[64][17];
+    const int c = blockIdx.x * 16 + (threadIdx.x & 15);
+    const bool which = blockIdx.y != 0;
+    if (!(which ? partF : partE)) return;
+    const float v = column_sum(which ? partF : partE, which ? nF : nE, (long)(which ? 1 : strideE) * D, c, D, sh);
+    if (threadIdx.x >= 16 || c >= D) return;
+    if (which) { if (dw_next) dw_next[c] = v; }
+    else {
+        if (dw_post) dw_post[c] = v * (scale ? scale[c] : 1.f);
+        if (dscale) dscale[c] = v * w_post[c];
     }
 }
 
@@ -292,7 +343,7 @@ bool vec8(int D, const NormArgs& a) {
 }
 int tpr_of(int D, int per) {                // threads a row: the fewest wavefronts whose registers hold it
     int t = 64;
-    while (t < 512 && (long)t * per < D) t <<= 1;
+    while (t < 1024 && (long)t * per < D) t <<= 1;
     return t;
 }
 int check(const NormArgs& a, int xdt, int udt, int gmode) {
@@ -301,22 +352,27 @@ int check(const NormArgs& a, int xdt, int udt, int gmode) {
     if (!a.x || (a.u && !a.w_post) || (gmode && (!a.gate || !a.u)) || (!a.u && !a.w_next)) return -1003;
     return 0;
 }
-int segments(long B, long T) { return B >= MAXB ? 1 : (int)min((MAXB + B - 1) / B, T); }
-
 template <typename XT, typename UT>
 void launch(NormArgs& a, bool bwd, hipStream_t st, int& blocks) {
     const bool v8 = vec8(a.D, a);
-    const int per = a.D <= 4096 ? 8 : (a.D <= 8192 ? 16 : 32);
+    const int per = a.D <= 8192 ? 8 : 16;
     a.tpr = tpr_of(a.D, per);
     const int threads = a.tpr == 64 ? 256 : a.tpr, rpb = threads / a.tpr;
-    if (!bwd) blocks = (int)min((a.rows + rpb - 1) / rpb, (long)MAXB * 1024 / threads);
-    else {
-        if (a.gmode != 2) a.items = (int)min((a.rows + rpb - 1) / rpb, (long)MAXB);
-        blocks = min(a.items, MAXB);
+    const long fit = min((long)MAXB, 256L * 1024 / threads);             // blocks that the chip holds at once
+    blocks = (int)min((a.rows + rpb - 1) / rpb, fit);
+    if (bwd) {
+        a.items = blocks;
+        if (a.gmode == 2) {
+            const long B = a.rows / a.T;
+            a.S = B >= fit ? 1 : (int)min((fit + B - 1) / B, a.T);
+            a.items = (int)(B * a.S);
+            blocks = (int)min((long)a.items, fit);
+        }
+        if (a.partF) a.partF = a.partE0 + (a.partE ? (long)a.items * a.D : 0);
     }
 #define GO(V, N) (bwd ? norm_bwd_kernel<XT, UT, V, N><<<blocks, threads, 0, st>>>(a) : norm_fwd_kernel<XT, UT, V, N><<<blocks, threads, 0, st>>>(a))
-    if (v8) per == 8 ? GO(8, 1) : per == 16 ? GO(8, 2) : GO(8, 4);
-    else per == 8 ? GO(1, 8) : per == 16 ? GO(1, 16) : GO(1, 32);
+    if (v8) per == 8 ? GO(8, 1) : GO(8, 2);
+    else per == 8 ? GO(1, 8) : GO(1, 16);
 #undef GO
 }
 void dispatch(NormArgs& a, int xdt, int udt, bool bwd, hipStream_t st, int& blocks) {
@@ -358,22 +414,24 @@ extern "C" int cpcsv_norm_residual_bwd(const void* x, const void* u, const void*
     const bool needE = u && (dscale || dw_post || (gate_mode == 2 && dgate)), needF = dw_next && a.dz;
     if (!dx || (u && !ru) || (a.dz && !rx) || ((needE || needF) && !part)) return -1003;
     const long B = gate_mode == 2 ? rows / T : 0;
-    if (gate_mode == 2) { a.S = segments(B, T); a.items = (int)(B * a.S); }
-    const long itemsMax = gate_mode == 2 ? B * a.S : MAXB;
+    a.partE0 = part;                          // E's rows (an item each), then F's (a block each)
     if (needE) a.partE = part;
-    if (needF) a.partF = part + itemsMax * D;
+    if (needF) a.partF = part;
     hipStream_t st = (hipStream_t)stream;
     int blocks = 0;
     dispatch(a, xdt, udt, true, st, blocks);
     CPCSV_CHECK_LAUNCH();
     if (needE && gate_mode == 2) {
-        const int n = cdiv(B * D, 256);
-        if (udt == CPCSV_F32) norm_gate_kernel<float><<<n, 256, 0, st>>>((const float*)gate, scale, w_post, part, (float*)dgate, (int)B, a.S, D);
-        else norm_gate_kernel<bf16_t><<<n, 256, 0, st>>>((const bf16_t*)gate, scale, w_post, part, (bf16_t*)dgate, (int)B, a.S, D);
+        for (long b0 = 0; b0 < B; b0 += 65535) {                          // (the grid's second dimension)
+            const dim3 n(cdiv(D, 16), (unsigned)min(65535L, B - b0));
+            float* e = part + b0 * a.S * D;
+            if (udt == CPCSV_F32) norm_gate_kernel<float><<<n, 1024, 0, st>>>((const float*)gate + b0 * D, scale, w_post, e, dgate ? (float*)dgate + b0 * D : nullptr, a.S, D);
+            else norm_gate_kernel<bf16_t><<<n, 1024, 0, st>>>((const bf16_t*)gate + b0 * D, scale, w_post, e, dgate ? (bf16_t*)dgate + b0 * D : nullptr, a.S, D);
+        }
         CPCSV_CHECK_LAUNCH();
     }
     if ((needE && (dscale || dw_post)) || needF) {
-        norm_cols_kernel<<<cdiv(D, 32), 1024, 0, st>>>(a.partE, gate_mode == 2 ? (int)B : blocks, gate_mode == 2 ? a.S : 1, a.partF, blocks,
+        norm_cols_kernel<<<dim3(cdiv(D, 16), 2), 1024, 0, st>>>(needE ? part : nullptr, gate_mode == 2 ? (int)B : blocks, gate_mode == 2 ? a.S : 1, a.partF, blocks,
                                                        scale, w_post, dscale, dw_post, dw_next, D);
         CPCSV_CHECK_LAUNCH();
     }
