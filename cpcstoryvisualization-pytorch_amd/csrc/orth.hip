@@ -37,7 +37,7 @@ constexpr int PAD = 128, MAXJ = CPCSV_ORTH_JOBS, MAXT = 2 * MAXJ, NORMB = 1024; 
 
 struct Job {
     const void* g; float* m; void* out;       // gradient, momentum (NULL: none), weight or result
-    long x, xt;                               // offsets of the hi planes in halves; the lo plane follows each
+    long x, xt;                               // offsets in halves
     int rows, cols;                           // of the matrix
     int M, N, tall;                           // padded min / max side; tall: rows > cols
     int t_norm, t_split;                      // first block of the job
@@ -64,6 +64,10 @@ __device__ __forceinline__ uint32_t split_of(float v) {           // hi | lo << 
     p.h[1] = (_Float16)(v - (float)p.h[0]);
     return p.w;
 }
+// An operand [rows][K] holds, of each row, 32 values' hi halves and then their lo halves, 128 bytes: a slice of 32 K is a cache line
+// (planes apart, a product of 128 x 128 tiles asked for half lines and was bound by them: 64-byte rows 0.65 us for 32 KB a CU, 128-byte
+// rows 0.43). Offset of (r, k)'s hi half; lo is 32 further.
+__device__ __forceinline__ long at_of(long r, int k, int K) { return r * 2 * K + (k >> 5) * 64 + (k & 31); }
 __device__ __forceinline__ void planes_of(const uint32_t* w, half8& hi, half8& lo) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -168,7 +172,6 @@ __global__ __launch_bounds__(256) void orth_split_kernel(Jobs s) {
     }
     __syncthreads();
     _Float16 *own = s.ws + (j.tall ? j.xt : j.x), *turned = s.ws + (j.tall ? j.x : j.xt);
-    const long plane = (long)j.M * j.N;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int line = i * 32 + (threadIdx.x >> 3), q = (threadIdx.x & 7) * 8;
@@ -179,9 +182,9 @@ __global__ __launch_bounds__(256) void orth_split_kernel(Jobs s) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] = way ? t[q + e][line] : t[line][q + e];
             planes_of(w, hi, lo);
-            _Float16* d = way ? turned + (long)(c0 + line) * PR + r0 + q : own + (long)(r0 + line) * PC + c0 + q;
+            _Float16* d = way ? turned + at_of(c0 + line, r0 + q, PR) : own + at_of(r0 + line, c0 + q, PC);
             *(half8*)d = hi;
-            *(half8*)(d + plane) = lo;
+            *(half8*)(d + 32) = lo;
         }
     }
 }
@@ -189,11 +192,11 @@ __global__ __launch_bounds__(256) void orth_split_kernel(Jobs s) {
 // ---- the products: D = alpha P Q^T + beta E + gamma I over two-plane operands [rows][K] ------------------------------
 enum { SYMM, BOTH, OUT };      // D symmetric: lower triangle and its mirror image | D and its transpose | the result or the weight
 struct Task {
-    long p, q, e, d, dt;       // offsets of the hi planes in halves (e < 0: none); OUT: d is the output's address
+    long p, q, e, d, dt;       // offsets in halves (e < 0: none); OUT: d is the output's address
     long slab;                 // first partial tile, in floats
     int R, C, K;
     float alpha, beta, gamma;
-    int kind, t0, tiles, whole, S, r0;        // first block; tiles, of which `whole` in one piece, the others in S slices of K; first joining block
+    int kind, shape, t0, tiles, whole, S, r0; // tile shape; first block; tiles, of which `whole` in one piece, the others in S slices of K; first joining block
     int rows, cols, tall;                     // OUT: of the output
 };
 struct Launch {
@@ -212,8 +215,9 @@ struct Launch {
 // block a wavefront keeps two accumulators (a chain of dependent MFMAs half as long) and has its entries of E loaded beforehand
 // (512^3: 6.7 us for the bare product against 13.3 and 34).
 template <int BM_, int WM_, int WN_, int BK_> struct Cfg {
-    static constexpr int BM = BM_, WM = WM_, WN = WN_, BK = BK_, WC = BM / WN, NW = (BM / WM) * WC, T = NW * 64, CPR = BK / 8;
-    static constexpr int LD = BM * CPR / T;                       // 16-byte loads a thread, operand plane and stage
+    static constexpr int BM = BM_, WM = WM_, WN = WN_, BK = BK_, WC = BM / WN, NW = (BM / WM) * WC, T = NW * 64;
+    static constexpr int CPR = BK / 4;                            // 16-byte chunks of a row's slice, both halves
+    static constexpr int LD = BM * CPR / T;                       // loads a thread, operand and stage
     static constexpr int STAGE = 4 * BM * BK;                     // halves
     static constexpr int SW = WN < 64 ? WN : 64, NB = SW / 32;    // columns of an epilogue strip, their 32 x 32 blocks
     static constexpr int STRIP = 32 * (SW + 1);                   // words of a strip in LDS
@@ -221,7 +225,7 @@ template <int BM_, int WM_, int WN_, int BK_> struct Cfg {
     static constexpr int MA = WM / 32, MB = WN / 32, STRIPS = MA * MB / NB;
     // chunk (16 bytes) q of LDS row r lives in slot q ^ swz(r): the rows a fragment read touches together fall into all banks. The
     // DMA writes LDS in lane order, so the permutation is on the source side.
-    static __device__ __forceinline__ int swz(int r) { return CPR == 4 ? (r >> 2) & 3 : (r >> 1) & 7; }
+    static __device__ __forceinline__ int swz(int r) { return CPR == 8 ? (r >> 1) & 7 : r & 15; }
 };
 using Big = Cfg<256, 128, 64, 32>;
 using Mid = Cfg<128, 64, 64, 32>;
@@ -258,11 +262,11 @@ template <int N, typename F> __device__ __forceinline__ void static_for(F&& f) {
     }
 }
 
-__device__ __forceinline__ uint32_t entry(const Launch& s, const Task& t, int r, int c, long RC) {     // of E, hi | lo << 16
+__device__ __forceinline__ uint32_t entry(const Launch& s, const Task& t, int r, int c) {               // of E, hi | lo << 16
     union { uint32_t w; _Float16 h[2]; } p;
-    const _Float16* o = s.ws + t.e + (long)r * t.C + c;
+    const _Float16* o = s.ws + t.e + at_of(r, c, t.C);
     p.h[0] = o[0];
-    p.h[1] = o[RC];
+    p.h[1] = o[32];
     return p.w;
 }
 
@@ -275,7 +279,6 @@ __device__ __forceinline__ void finish(const Launch& s, const Task& t, int r0, i
     const int lane = threadIdx.x & 63, fr = lane & 31, fk = lane >> 5;
     if (r0 >= t.R || c0 >= t.C || (t.kind == SYMM && r0 + 31 < c0)) return;                // (sides are multiples of a strip's)
     const bool diag = t.kind == SYMM && r0 < c0 + SW;                                      // the strip meets the diagonal
-    const long RC = (long)t.R * t.C;
     const float lr = t.kind == OUT && s.hyper ? s.hyper[0] : 0.f;
     const float keep = 1.f - lr * s.decay, step = lr * sqrtf(fmaxf(1.f, (float)t.rows / (float)t.cols));
     asm volatile("" ::: "memory");               // (the next strip's loads are not hoisted over this one: they would not fit the registers)
@@ -290,7 +293,7 @@ __device__ __forceinline__ void finish(const Launch& s, const Task& t, int r0, i
             if (t.e >= 0) {
                 union { uint32_t w; _Float16 h[2]; } p;
                 if (EARLY) p.w = early[i];                    // (one block a strip)
-                else p.w = entry(s, t, r, c, RC);
+                else p.w = entry(s, t, r, c);
                 v += ((float)p.h[0] + (float)p.h[1]) * t.beta + (r == c ? t.gamma : 0.f);
             }
             buf[rl * LDW + cl] = t.kind == OUT ? __float_as_uint(v) : split_of(v);
@@ -340,16 +343,16 @@ __device__ __forceinline__ void finish(const Launch& s, const Task& t, int r0, i
 #pragma unroll
                 for (int e = 0; e < 8; ++e) w[e] = cb == r0 && line < q + e ? z[(q + e) * LDW + line] : z[line * LDW + q + e];
                 planes_of(w, hi, lo);
-                _Float16* d = s.ws + t.d + (long)(r0 + line) * t.C + cb + q;
+                _Float16* d = s.ws + t.d + at_of(r0 + line, cb + q, t.C);
                 *(half8*)d = hi;
-                *(half8*)(d + RC) = lo;
+                *(half8*)(d + 32) = lo;
                 if (cb == r0) continue;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) w[e] = z[(q + e) * LDW + line];
                 planes_of(w, hi, lo);
-                d = s.ws + t.d + (long)(cb + line) * t.C + r0 + q;
+                d = s.ws + t.d + at_of(cb + line, r0 + q, t.C);
                 *(half8*)d = hi;
-                *(half8*)(d + RC) = lo;
+                *(half8*)(d + 32) = lo;
             }
         }
         return;
@@ -363,9 +366,9 @@ __device__ __forceinline__ void finish(const Launch& s, const Task& t, int r0, i
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = buf[rl * LDW + cl + e];
         planes_of(w, hi, lo);
-        _Float16* d = s.ws + t.d + (long)(r0 + rl) * t.C + c0 + cl;
+        _Float16* d = s.ws + t.d + at_of(r0 + rl, c0 + cl, t.C);
         *(half8*)d = hi;
-        *(half8*)(d + RC) = lo;
+        *(half8*)(d + 32) = lo;
     }
     _Float16* const turned = s.ws + (t.kind == SYMM ? t.d : t.dt);                 // (D^T [C][R]; R = C for a symmetric one)
 #pragma unroll
@@ -374,24 +377,22 @@ __device__ __forceinline__ void finish(const Launch& s, const Task& t, int r0, i
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = buf[(rl + e) * LDW + cl];
         planes_of(w, hi, lo);
-        _Float16* d = turned + (long)(c0 + cl) * t.R + r0 + rl;
+        _Float16* d = turned + at_of(c0 + cl, r0 + rl, t.R);
         *(half8*)d = hi;
-        *(half8*)(d + RC) = lo;
+        *(half8*)(d + 32) = lo;
     }
 }
 
-template <typename C>
-__global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    _Float16* const lds = (_Float16*)smem;
+__device__ __forceinline__ const Task& task_of(const Launch& s) {
+    if (s.n == 1) return s.t[0];
     // (all first blocks compared at once: a search would be a chain of dependent loads)
-    const int lane = threadIdx.x & 63;
-    int k = 0;
-    if (s.n > 1) {
-        const int first = s.t[min(lane, s.n - 1)].t0;
-        k = __popcll(__ballot(lane < s.n && (int)blockIdx.x >= first)) - 1;
-    }
-    const Task& t = s.t[k];
+    const int lane = threadIdx.x & 63, first = s.t[min(lane, s.n - 1)].t0;
+    return s.t[__popcll(__ballot(lane < s.n && (int)blockIdx.x >= first)) - 1];
+}
+
+template <typename C>
+__device__ __forceinline__ void product(const Launch& s, const Task& t, unsigned char* smem) {
+    _Float16* const lds = (_Float16*)smem;
     // the whole tiles first, then the others, slice by slice. Blocks go to the eight XCDs in turn: each gets a contiguous run of
     // either part, whose operands its L2 then holds, and a share of both
     const bool sliced = (int)blockIdx.x - t.t0 >= t.whole;
@@ -401,10 +402,9 @@ __global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
     const int S = sliced ? t.S : 1, sl = sliced ? u / cut : 0, tile = sliced ? t.whole + u % cut : u;
     int ti, tj;
     tile_of(t, tile, C::BM, ti, tj);
-    const int tid = threadIdx.x, wave = tid >> 6, K = t.K;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, K = t.K;
     const int nk = K / C::BK, k0 = (int)((long)nk * sl / S), k1 = (int)((long)nk * (sl + 1) / S);
-    const _Float16* src[2] = {s.ws + t.p + (long)ti * C::BM * K, s.ws + t.q + (long)tj * C::BM * K};
-    const long pl[2] = {(long)t.R * K, (long)t.C * K};
+    const _Float16* src[2] = {s.ws + t.p + (long)ti * C::BM * 2 * K, s.ws + t.q + (long)tj * C::BM * 2 * K};
     int off[2][C::LD];                           // (K <= 131072 and 256 rows: below 2^31)
 #pragma unroll
     for (int o = 0; o < 2; ++o)
@@ -412,18 +412,16 @@ __global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
         for (int i = 0; i < C::LD; ++i) {
             const int idx = i * C::T + tid, row = idx / C::CPR, q = (idx % C::CPR) ^ C::swz(row);
             const int last = (o ? t.C - tj * C::BM : t.R - ti * C::BM) - 1;               // a tile may hang over the padded side
-            off[o][i] = min(row, last) * K + q * 8;
+            off[o][i] = min(row, last) * 2 * K + q * 8;
         }
     auto stage = [&](int buf, int kt) {
 #pragma unroll
         for (int o = 0; o < 2; ++o)
 #pragma unroll
-            for (int p = 0; p < 2; ++p)
-#pragma unroll
-                for (int i = 0; i < C::LD; ++i)
-                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[o] + (p ? pl[o] : 0) + off[o][i] + kt * C::BK),
-                                                     (__attribute__((address_space(3))) void*)(lds + buf * C::STAGE + (o * 2 + p) * C::BM * C::BK +
-                                                                                               (i * C::T + wave * 64) * 8), 16, 0, 0);
+            for (int i = 0; i < C::LD; ++i)
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[o] + off[o][i] + (long)kt * 2 * C::BK),
+                                                 (__attribute__((address_space(3))) void*)(lds + buf * C::STAGE + o * C::BM * 2 * C::BK +
+                                                                                           (i * C::T + wave * 64) * 8), 16, 0, 0);
     };
     const int wm = wave / C::WC * C::WM, wn = wave % C::WC * C::WN, fr = lane & 31, fk = lane >> 5;
     f32x16 acc[C::MA][C::MB], low;               // low: the hi lo terms of a one-block wavefront
@@ -442,7 +440,7 @@ __global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
         const int r0 = ti * C::BM + wm, c0 = tj * C::BM + wn;
         if (r0 < t.R && c0 < t.C)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) early[i] = entry(s, t, r0 + (i >> 2) * 8 + fk * 4 + (i & 3), c0 + fr, (long)t.R * t.C);
+            for (int i = 0; i < 16; ++i) early[i] = entry(s, t, r0 + (i >> 2) * 8 + fk * 4 + (i & 3), c0 + fr);
     }
     for (int kt = k0; kt < k1; ++kt) {
         const int buf = (kt - k0) & 1;
@@ -458,12 +456,12 @@ __global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
 #pragma unroll
                 for (int a = 0; a < C::MA; ++a) {
                     const int row = wm + a * 32 + fr;
-                    fp[p][a] = *(const half8*)(base + p * C::BM * C::BK + row * C::BK + ((kk * 2 + fk) ^ C::swz(row)) * 8);
+                    fp[p][a] = *(const half8*)(base + row * 2 * C::BK + (((kk >> 1) * 8 + p * 4 + (kk & 1) * 2 + fk) ^ C::swz(row)) * 8);
                 }
 #pragma unroll
                 for (int b = 0; b < C::MB; ++b) {
                     const int row = wn + b * 32 + fr;
-                    fq[p][b] = *(const half8*)(base + (2 + p) * C::BM * C::BK + row * C::BK + ((kk * 2 + fk) ^ C::swz(row)) * 8);
+                    fq[p][b] = *(const half8*)(base + (C::BM + row) * 2 * C::BK + (((kk >> 1) * 8 + p * 4 + (kk & 1) * 2 + fk) ^ C::swz(row)) * 8);
                 }
             }
 #define FOR_ACC for (int a = 0; a < C::MA; ++a) _Pragma("unroll") for (int b = 0; b < C::MB; ++b)
@@ -505,12 +503,20 @@ __global__ __launch_bounds__(C::T) void orth_gemm_kernel(Launch s) {
     });
 }
 
+// one launch serves the two shapes of 256 threads and 64 KB of LDS
+__global__ __launch_bounds__(Mid::T) void orth_gemm_kernel(Launch s) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const Task& t = task_of(s);
+    if (t.shape == 1) product<Mid>(s, t, smem);
+    else product<Small>(s, t, smem);
+}
+__global__ __launch_bounds__(Big::T) void orth_gemm_big_kernel(Launch s) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    product<Big>(s, task_of(s), smem);
+}
+
 // the slices of a tile, added in order: one wavefront a strip
-template <typename C>
-__global__ __launch_bounds__(64) void orth_join_kernel(Launch s) {
-    __shared__ uint32_t buf[C::STRIP];
-    const int first = s.t[min((int)threadIdx.x, s.n - 1)].r0;
-    const Task& t = s.t[__popcll(__ballot((int)threadIdx.x < s.n && (int)blockIdx.x >= first)) - 1];
+template <typename C> __device__ __forceinline__ void join(const Launch& s, const Task& t, uint32_t* buf) {
     const int id = blockIdx.x - t.r0, strip = id % (C::NW * C::STRIPS), cut = id / (C::NW * C::STRIPS), wave = strip / C::STRIPS;
     const int a = strip % C::STRIPS / (C::MB / C::NB), b = strip % (C::MB / C::NB) * C::NB;
     int ti, tj;
@@ -533,6 +539,15 @@ __global__ __launch_bounds__(64) void orth_join_kernel(Launch s) {
             }
     finish<C, false>(s, t, ti * C::BM + wave / C::WC * C::WM + a * 32, tj * C::BM + wave % C::WC * C::WN + b * 32, acc, buf, u32x16{});
 }
+__global__ __launch_bounds__(64) void orth_join_kernel(Launch s) {
+    __shared__ uint32_t buf[Mid::STRIP];
+    const int first = s.t[min((int)threadIdx.x, s.n - 1)].r0;
+    const Task& t = s.t[__popcll(__ballot((int)threadIdx.x < s.n && (int)blockIdx.x >= first)) - 1];
+    if (t.shape == 0) join<Big>(s, t, buf);
+    else if (t.shape == 1) join<Mid>(s, t, buf);
+    else join<Small>(s, t, buf);
+}
+static_assert(Mid::T == Small::T && Mid::LDS == Small::LDS && Mid::STRIP >= Small::STRIP && Mid::STRIP >= Big::STRIP, "shared launches");
 
 // ---- host: the schedule ---------------------------------------------------------------------------------------------
 long tiles_of(int kind, long R, long C, int bm) {
@@ -543,8 +558,9 @@ long tiles_of(int kind, long R, long C, int bm) {
 // (all of them, where there are few: 1024 x 18432 against itself has 36 of 128 x 128 and took 470 us in one piece). By the
 // product's sides alone, so that a matrix has the same bits in any company. Least time by what a K step was measured to take (us;
 // `two`: while two blocks share the CU) and a block's fixed part; a join reads and writes its slabs once.
-struct Shape { int bm, bk, fit; double one, two, fixed; };
-constexpr Shape SHAPES[3] = {{256, 32, 1, 2.5, 2.5, 30.0}, {128, 32, 2, 0.9, 1.6, 10.0}, {64, 64, 2, 0.57, 1.14, 7.0}};
+struct Shape { int bm, bk, fit, strips; double one, two, fixed; };
+constexpr Shape SHAPES[3] = {{256, 32, 1, Big::NW * Big::STRIPS, 2.5, 2.5, 30.0}, {128, 32, 2, Mid::NW * Mid::STRIPS, 0.9, 1.6, 10.0},
+                             {64, 64, 2, Small::NW * Small::STRIPS, 0.57, 1.14, 7.0}};
 struct Cut { int shape, whole, S; long slab; };               // slab: floats
 Cut cut_of(int kind, long R, long C, long K) {
     Cut best{0, 0, 1, 0};
@@ -602,47 +618,37 @@ int plan(Jobs& s, Scratch* sc, const long* dims, int njobs, Plan& p) {
     return 0;
 }
 
-template <typename C> int go(Launch& s, hipStream_t st) {
-    if (!s.n) return 0;
-    long units = 0, joins = 0;
-    Launch only = s;                                            // the sliced products alone
-    only.n = 0;
-    for (int i = 0; i < s.n; ++i) {
-        Task& t = s.t[i];
-        t.t0 = (int)units; t.r0 = (int)joins;
-        units += t.whole + (long)(t.tiles - t.whole) * t.S;
-        if (t.S > 1) {
-            joins += (long)(t.tiles - t.whole) * C::NW * C::STRIPS;
-            only.t[only.n++] = t;
-        }
-        if (units > (1L << 30) || joins > (1L << 30)) return -1002;
-    }
-    if (C::LDS > 64 * 1024) {                                   // more than the default cap of dynamic LDS: raise it once
-        static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(orth_gemm_kernel<C>), hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
-        if (e != hipSuccess) return -(int)e;
-    }
-    orth_gemm_kernel<C><<<(int)units, C::T, C::LDS, st>>>(s);
-    if (joins) orth_join_kernel<C><<<(int)joins, 64, 0, st>>>(only);
-    CPCSV_CHECK_LAUNCH();
-    return 0;
-}
-// the products of one level, a launch for each tile shape among them
+// the products of one level: a launch for those of the big tile, one for the others, one that joins slices
 int run_level(const Launch& all, long slabs, hipStream_t st) {
-    long at = 0;
-    Launch by[3];
-    for (int c = 0; c < 3; ++c) { by[c] = all; by[c].n = 0; }
+    Launch big = all, rest = all, join = all;
+    big.n = rest.n = join.n = 0;
+    long at = 0, units[2] = {0, 0}, joins = 0;
     for (int i = 0; i < all.n; ++i) {
         Task t = all.t[i];
         const Cut cut = cut_of(t.kind, t.R, t.C, t.K);
+        t.shape = cut.shape;
         t.tiles = (int)tiles_of(t.kind, t.R, t.C, SHAPES[cut.shape].bm);
         t.whole = cut.whole; t.S = cut.S; t.slab = at;
         at += cut.slab;
-        by[cut.shape].t[by[cut.shape].n++] = t;
+        long& u = units[cut.shape != 0];
+        t.t0 = (int)u; t.r0 = (int)joins;
+        u += t.whole + (long)(t.tiles - t.whole) * t.S;
+        if (t.S > 1) joins += (long)(t.tiles - t.whole) * SHAPES[cut.shape].strips;
+        if (u > (1L << 30) || joins > (1L << 30)) return -1002;
+        Launch& to = cut.shape ? rest : big;
+        to.t[to.n++] = t;
+        if (t.S > 1) join.t[join.n++] = t;
     }
     if (at > slabs) return -1004;
-    if (int rc = go<Big>(by[0], st)) return rc;
-    if (int rc = go<Mid>(by[1], st)) return rc;
-    return go<Small>(by[2], st);
+    if (big.n) {                                                // more than the default cap of dynamic LDS: raise it once
+        static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(orth_gemm_big_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, Big::LDS);
+        if (e != hipSuccess) return -(int)e;
+        orth_gemm_big_kernel<<<(int)units[0], Big::T, Big::LDS, st>>>(big);
+    }
+    if (rest.n) orth_gemm_kernel<<<(int)units[1], Mid::T, Mid::LDS, st>>>(rest);
+    if (join.n) orth_join_kernel<<<(int)joins, 64, 0, st>>>(join);
+    CPCSV_CHECK_LAUNCH();
+    return 0;
 }
 
 int iterate(Jobs& s, const Scratch* sc, const Plan& p, int steps, const float* hyper, float decay, void* ws, hipStream_t st) {
