@@ -568,3 +568,70 @@ class GRUCell(nn.Module):
 
     def forward(self, x, h):
         return self.step(self.input_gates(x), h)
+
+
+# ------------------------------------------------------------------------------------------------
+# gated recurrent block: norm - projection - gated scan - projection - norm, gate, residual
+# ------------------------------------------------------------------------------------------------
+class GatedRecurrence(nn.Module):
+    """A recurrence beside GRUCell whose gates see the input only, so that a whole sequence is one projection and one scan
+    (cpcsv.functional.gated_scan): f | v | o = W x + b;  z = sigmoid(f);  h_t = z h_{t-1} + (1 - z) v;  y_t = h_t silu(o)
+    (out_gate=False: y = h). Inputs [B, T, input_size] (any strides of B and T), state fp32 [B, H]. The projection runs like every
+    dense layer here (exact fp32 for small ones, the compute dtype otherwise) and decides the type of y. The bias of f starts at +2:
+    a memory of some ten tokens."""
+
+    def __init__(self, input_size, hidden_size, out_gate=True):
+        super().__init__()
+        self.input_size, self.hidden_size, self.out_gate = input_size, hidden_size, bool(out_gate)
+        self.proj = Linear(input_size, (3 if out_gate else 2) * hidden_size)
+        with torch.no_grad():
+            self.proj.bias[:hidden_size] += 2.0
+
+    def project(self, x):
+        """x [..., input_size] -> p [..., 3H or 2H], the input of gated_scan / gated_scan_step."""
+        lay = _layer_for(self.proj, None, L.ACT_NONE, 0, out_mode="T")
+        rows = x.reshape(-1, self.input_size)
+        if rows.dtype != lay.in_dtype() or rows.shape[1] != lay.k_stored:
+            rows = rows.float()
+        return lay(rows).view(x.shape[:-1] + (pad8(self.proj.cout),))[..., :self.proj.cout]
+
+    def forward(self, x, h0=None, lengths=None):
+        """-> (y [B, T, H], h_last fp32 [B, H]); lengths int32 [B]: see gated_scan."""
+        if x.dim() != 3 or x.shape[2] != self.input_size:
+            raise ValueError("GatedRecurrence expects [B, T, %d], got %s" % (self.input_size, tuple(x.shape)))
+        return F.gated_scan(self.project(x), h0, lengths=lengths, out_gate=self.out_gate)
+
+    def step(self, x, h):
+        """One token: x [B, input_size], h fp32 [B, H] updated in place -> y [B, H] (no gradients)."""
+        if x.dim() != 2 or x.shape[1] != self.input_size:
+            raise ValueError("GatedRecurrence.step expects [B, %d], got %s" % (self.input_size, tuple(x.shape)))
+        with torch.no_grad():
+            return F.gated_scan_step(self.project(x), h, out_gate=self.out_gate)
+
+
+class RMSNorm(nn.Module):
+    """weight * x / sqrt(mean x^2 + eps) over the last dimension (cpcsv.functional.rms_norm): the norm before a first block."""
+
+    def __init__(self, dim, eps=1e-6):
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(dim))
+
+    def forward(self, x, out_dtype=None):
+        return F.rms_norm(x, self.weight, self.eps, out_dtype)
+
+
+class NormResidual(nn.Module):
+    """What stands between two blocks, one pass each way (cpcsv.functional.norm_residual): the norm of the block's output u, its gate,
+    a learned residual scale (scale=None: none; a number: its initial value), the residual sum, and the next block's norm
+    (last=True: none). forward(x, u, gate=None) -> (x', z), or x' for the last block."""
+
+    def __init__(self, dim, scale=None, last=False, eps=1e-6):
+        super().__init__()
+        self.eps = eps
+        self.weight_post = nn.Parameter(torch.ones(dim))
+        self.scale = nn.Parameter(torch.full((dim,), float(scale))) if scale is not None else None
+        self.weight_next = nn.Parameter(torch.ones(dim)) if not last else None
+
+    def forward(self, x, u, gate=None):
+        return F.norm_residual(x, u, self.weight_post, gate=gate, scale=self.scale, w_next=self.weight_next, eps=self.eps)
