@@ -1368,6 +1368,10 @@ class GruSeqFn(Function):
 # ------------------------------------------------------------------------------------------------
 # gated linear recurrence
 # ------------------------------------------------------------------------------------------------
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def _scan_args(p, h0, lengths, out_gate, rank):
     """Checks of gated_scan / gated_scan_step -> H."""
     k, shape = 3 if out_gate else 2, p.shape
@@ -1394,27 +1398,33 @@ def _scan_args(p, h0, lengths, out_gate, rank):
     return h
 
 
+def _scan_forward(p, h0, lengths, out_gate, keep):
+    """-> y, h_last, and what a backward pass needs: p, h0, lengths as the kernels read them, the chunk states (keep)"""
+    b, t, h = p.shape[0], p.shape[1], p.shape[2] // (3 if out_gate else 2)
+    if p.stride(2) != 1:
+        p = p.contiguous()
+    h0 = h0.contiguous() if h0 is not None else None
+    lengths = lengths.contiguous() if lengths is not None else None
+    dev = p.device
+    y = _empty((b, t, h), p.dtype, dev)
+    last = _empty((b, h), torch.float32, dev)
+    hin = None
+    if b == 0 or t == 0:
+        last.copy_(h0) if h0 is not None else last.zero_()
+    else:
+        if keep and K.scan_states(t):
+            hin = _empty((b, K.scan_states(t), h), torch.float32, dev)
+        ws = K.scan_fwd(p, h0, lengths, y, last, hin, b, t, h, out_gate)
+        _runtime.keep_forced(p, h0, lengths, hin, ws)
+    return y, last, p, h0, lengths, hin
+
+
 class GatedScanFn(Function):
     """(y, h_last) of the gated linear recurrence; see gated_scan."""
 
     @staticmethod
-    def forward(ctx, p, h0, lengths, out_gate, keep):
-        b, t, h = p.shape[0], p.shape[1], p.shape[2] // (3 if out_gate else 2)
-        if p.stride(2) != 1:
-            p = p.contiguous()
-        h0 = h0.contiguous() if h0 is not None else None
-        lengths = lengths.contiguous() if lengths is not None else None
-        dev = p.device
-        y = _empty((b, t, h), p.dtype, dev)
-        last = _empty((b, h), torch.float32, dev)
-        hin = None
-        if b == 0 or t == 0:
-            last.copy_(h0) if h0 is not None else last.zero_()
-        else:
-            if keep and K.scan_states(t):
-                hin = _empty((b, K.scan_states(t), h), torch.float32, dev)
-            ws = K.scan_fwd(p, h0, lengths, y, last, hin, b, t, h, out_gate)
-            _runtime.keep_forced(p, h0, lengths, hin, ws)
+    def forward(ctx, p, h0, lengths, out_gate):
+        y, last, p, h0, lengths, hin = _scan_forward(p, h0, lengths, out_gate, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(p, h0, lengths, hin)
         ctx.out_gate = out_gate
@@ -1426,19 +1436,19 @@ class GatedScanFn(Function):
         p, h0, lengths, hin = ctx.saved_tensors
         b, t, h = p.shape[0], p.shape[1], p.shape[2] // (3 if ctx.out_gate else 2)
         if dy is None and dlast is None:
-            return (None,) * 5
+            return (None,) * 4
         dev = p.device
         dp = _empty(p.shape, p.dtype, dev)
         dh0 = _empty((b, h), torch.float32, dev) if h0 is not None and ctx.needs_input_grad[1] else None
         if b == 0 or t == 0:
             if dh0 is not None:
                 dh0.copy_(dlast) if dlast is not None else dh0.zero_()
-            return dp, dh0, None, None, None
+            return dp, dh0, None, None
         dy = torch.zeros((b, t, h), dtype=p.dtype, device=dev) if dy is None else dy.contiguous()
         dlast = dlast.contiguous() if dlast is not None else None
         ws = K.scan_bwd(p, h0, lengths, hin, dy, dlast, dp, dh0, b, t, h, ctx.out_gate)
         _runtime.keep_forced(dy, dlast, ws)
-        return dp, dh0, None, None, None
+        return dp, dh0, None, None
 
 
 def gated_scan(p, h0=None, lengths=None, out_gate=True):
@@ -1450,8 +1460,9 @@ def gated_scan(p, h0=None, lengths=None, out_gate=True):
     without W_hh: the whole sequence is two launches however long it is (one up to 32 tokens, which then has the very bits of
     gated_scan_step token by token)."""
     _scan_args(p, h0, lengths, out_gate, 3)
-    keep = torch.is_grad_enabled() and (p.requires_grad or (h0 is not None and h0.requires_grad))
-    return GatedScanFn.apply(p, h0, lengths, bool(out_gate), keep)
+    if not _wants_grad(p, h0):
+        return _scan_forward(p, h0, lengths, bool(out_gate), False)[:2]
+    return GatedScanFn.apply(p, h0, lengths, bool(out_gate))
 
 
 def gated_scan_step(p, h, out_gate=True):
@@ -1473,33 +1484,39 @@ def gated_scan_step(p, h, out_gate=True):
 # ------------------------------------------------------------------------------------------------
 # norms around a block
 # ------------------------------------------------------------------------------------------------
+def _norm_forward(x, u, w_post, gate, scale, w_next, out_dtype, eps, keep):
+    """Forward of norm_residual / rms_norm (u None) -> outputs, tensors a backward pass needs, (rows, D, u's type, gate mode, tokens a gate)"""
+    d = x.shape[-1]
+    rows = x.numel() // d if d else 0
+    dev, udt = x.device, dcode(u) if u is not None else (L.F32 if out_dtype == torch.float32 else L.BF16)
+    x = x.contiguous()
+    u, gate, w_post, scale, w_next = (None if q is None else q.contiguous() for q in (u, gate, w_post, scale, w_next))
+    mode, t = 0, 1
+    if gate is not None:
+        per = gate.numel() // d if d else 0
+        mode, t = (1, 1) if per == rows else (2, rows // per)
+    xo = _empty(x.shape, x.dtype, dev) if u is not None else None
+    z = _empty(x.shape, out_dtype, dev) if w_next is not None else None
+    ru = rx = None
+    if rows:
+        if keep:
+            ru = _empty((rows,), torch.float32, dev) if u is not None else None
+            rx = _empty((rows,), torch.float32, dev) if w_next is not None else None
+        K.norm_residual_fwd(x, u, gate, scale, w_post, w_next, xo, z, ru, rx, rows, d, udt, mode, t, eps)
+        _runtime.keep_forced(x, u, gate, w_post, scale, w_next, ru, rx)
+    outs = (xo, z) if xo is not None and z is not None else (xo if xo is not None else z)
+    return outs, (x, u, w_post, gate, scale, w_next, ru, rx), (rows, d, udt, mode, t)
+
+
 class NormResidualFn(Function):
-    """Forward / backward of norm_residual and rms_norm (u None). x, u, gate: contiguous; gate [samples, D] or shaped like u."""
+    """Forward / backward of norm_residual and rms_norm (u None)."""
 
     @staticmethod
     def forward(ctx, x, u, w_post, gate, scale, w_next, out_dtype, eps):
-        d = x.shape[-1]
-        rows = x.numel() // d if d else 0
-        dev, udt = x.device, dcode(u) if u is not None else (L.F32 if out_dtype == torch.float32 else L.BF16)
-        x = x.contiguous()
-        u, gate = (None if q is None else q.contiguous() for q in (u, gate))
-        w_post, scale, w_next = (None if q is None else q.contiguous() for q in (w_post, scale, w_next))
-        mode, t = 0, 1
-        if gate is not None:
-            per = gate.numel() // d if d else 0
-            mode, t = (1, 1) if per == rows else (2, rows // per)
-        xo = _empty(x.shape, x.dtype, dev) if u is not None else None
-        z = _empty(x.shape, out_dtype, dev) if w_next is not None else None
-        ru = rx = None
-        if rows:
-            ru = _empty((rows,), torch.float32, dev) if u is not None else None
-            rx = _empty((rows,), torch.float32, dev) if w_next is not None else None
-            K.norm_residual_fwd(x, u, gate, scale, w_post, w_next, xo, z, ru, rx, rows, d, udt, mode, t, eps)
-            _runtime.keep_forced(x, u, gate, w_post, scale, w_next, ru, rx)
+        outs, saved, ctx.geom = _norm_forward(x, u, w_post, gate, scale, w_next, out_dtype, eps, True)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, u, w_post, gate, scale, w_next, ru, rx)
-        ctx.geom = (rows, d, udt, mode, t)
-        return (xo, z) if xo is not None and z is not None else (xo if xo is not None else z)
+        ctx.save_for_backward(*saved)
+        return outs
 
     @staticmethod
     @once_differentiable
@@ -1534,10 +1551,16 @@ class NormResidualFn(Function):
         return dx, du, dwp, dgate, dsc, dwn, None, None
 
 
+def _norm_call(*args):
+    if _wants_grad(*args[:6]):
+        return NormResidualFn.apply(*args)
+    return _norm_forward(*args, False)[0]
+
+
 def _norm_vec(name, w, d):
     if w.dtype != torch.float32:
         raise TypeError("%s must be float32, got %s" % (name, w.dtype))
-    if tuple(w.shape) != (d,):
+    if w.shape != (d,):
         raise ValueError("%s must have shape (%d,), got %s" % (name, d, tuple(w.shape)))
 
 
@@ -1558,7 +1581,7 @@ def rms_norm(x, weight, eps=1e-6, out_dtype=None):
     if out_dtype not in (torch.float32, torch.bfloat16) or (x.dtype == torch.bfloat16 and out_dtype == torch.float32):
         raise TypeError("out_dtype must be x's type or bfloat16, got %s of %s" % (out_dtype, x.dtype))
     _runtime.require_here(x, weight)
-    return NormResidualFn.apply(x, None, None, None, None, weight, out_dtype, float(eps))
+    return _norm_call(x, None, None, None, None, weight, out_dtype, float(eps))
 
 
 def norm_residual(x, u, w_post, gate=None, scale=None, w_next=None, eps=1e-6):
@@ -1586,7 +1609,7 @@ def norm_residual(x, u, w_post, gate=None, scale=None, w_next=None, eps=1e-6):
         if x.dim() == 1:
             raise ValueError("a gate needs x of at least two dimensions")
     _runtime.require_here(x, u, w_post, gate, scale, w_next)
-    return NormResidualFn.apply(x, u, w_post, gate, scale, w_next, u.dtype, float(eps))
+    return _norm_call(x, u, w_post, gate, scale, w_next, u.dtype, float(eps))
 
 
 class DynFilter1dFn(Function):

@@ -152,7 +152,7 @@ __global__ __launch_bounds__(1024) void norm_fwd_kernel(NormArgs a) {
 #pragma unroll
             for (int i = 0; i < E; ++i) x1[i] = residual(cur.x.at(i), a.gmode ? cur.g.at(i) : 1.f, w.f[i], __fmul_rn(cur.u.at(i), ru));
             store_row<XT, VEC, NV>(a.xo, row * a.D, x1, a, lr, on);
-            if (on && lr == 0) a.ru[row] = ru;
+            if (on && lr == 0 && a.ru) a.ru[row] = ru;
         } else {
 #pragma unroll
             for (int i = 0; i < E; ++i) x1[i] = cur.x.at(i);
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(1024) void norm_fwd_kernel(NormArgs a) {
 #pragma unroll
             for (int i = 0; i < E; ++i) x1[i] = x1[i] * rx * w.wn[i];
             store_row<UT, VEC, NV>(a.z, row * a.D, x1, a, lr, on);
-            if (on && lr == 0) a.rx[row] = rx;
+            if (on && lr == 0 && a.rx) a.rx[row] = rx;
         }
         if (AHEAD) cur = next;
     }
@@ -389,7 +389,7 @@ extern "C" int cpcsv_norm_residual_fwd(const void* x, const void* u, const void*
     a.x = x; a.u = u; a.gate = gate; a.scale = scale; a.w_post = w_post; a.w_next = w_next; a.xo = xo; a.z = z; a.ru = ru; a.rx = rx;
     a.rows = rows; a.D = D; a.gmode = gate_mode; a.T = T; a.eps = eps;
     if (int rc = check(a, xdt, udt, gate_mode)) return rc;
-    if ((u && (!xo || !ru)) || (w_next && (!z || !rx))) return -1003;
+    if ((u && !xo) || (w_next && !z)) return -1003;
     int blocks = 0;
     dispatch(a, xdt, udt, false, (hipStream_t)stream, blocks);
     CPCSV_CHECK_LAUNCH();

@@ -752,7 +752,7 @@ int cpcsv_scan_bwd(const void* p, int dtype, long psb, long pst, const float* h0
  *   x, xo    [rows][D] xdt, the residual stream    u, z, gate [rows][D] udt; (xdt, udt) = both fp32, both bf16, or fp32 with bf16.
  *   u NULL: z = w_next * x / rms(x) alone (xo, gate, scale, w_post unused); w_next NULL: no z.
  *   gate_mode  0 none, 1 one row for each row, 2 gate [rows / T][D]: one row for T consecutive rows (T divides rows)
- *   scale, w_post, w_next  fp32 [D]; scale NULL = 1        ru, rx  fp32 [rows]: 1/rms, written forward, read backward
+ *   scale, w_post, w_next  fp32 [D]; scale NULL = 1        ru, rx  fp32 [rows]: 1/rms, written forward (NULL: not), read backward
  *   dxo (NULL = 0), dx xdt; dz (NULL = 0), du, dgate udt; dscale, dw_post, dw_next fp32 [D]; each result but dx may be NULL
  *   part     fp32 workspace of cpcsv_norm_residual_part(...) values, needed when a weight's or a shared gate's gradient is asked for
  * D up to CPCSV_NORM_MAX_D. Contiguous tensors. No atomics: results do not depend on the run. */

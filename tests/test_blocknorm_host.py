@@ -56,12 +56,12 @@ def test_entry_points_reject_bad_arguments():
     header = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "cpcsv_hip.h")).read()
     assert int(re.search(r"#define CPCSV_NORM_MAX_D (\d+)", header).group(1)) == _lib.NORM_MAX_D
     p = 0x1000
-    fwd = lambda x=p, u=p, gate=None, wp=p, wn=p, rows=4, d=8, xdt=0, udt=0, mode=0, t=1, ru=p: lib.cpcsv_norm_residual_fwd(
-        x, u, gate, None, wp, wn, p, p, ru, p, rows, d, xdt, udt, mode, t, 1e-6, None)
+    fwd = lambda x=p, u=p, gate=None, wp=p, wn=p, rows=4, d=8, xdt=0, udt=0, mode=0, t=1, xo=p, z=p: lib.cpcsv_norm_residual_fwd(
+        x, u, gate, None, wp, wn, xo, z, p, p, rows, d, xdt, udt, mode, t, 1e-6, None)
     assert fwd(xdt=1, udt=0) == -1001 and fwd(udt=5) == -1001
     assert fwd(rows=0) == -1002 and fwd(d=0) == -1002 and fwd(d=16385) == -1002 and fwd(mode=3) == -1002
     assert fwd(mode=2, gate=p, t=3) == -1002 and fwd(mode=2, gate=p, t=0) == -1002
-    assert fwd(x=None) == -1003 and fwd(wp=None) == -1003 and fwd(mode=1) == -1003 and fwd(u=None, wn=None) == -1003 and fwd(ru=None) == -1003
+    assert fwd(x=None) == -1003 and fwd(wp=None) == -1003 and fwd(mode=1) == -1003 and fwd(u=None, wn=None) == -1003 and fwd(xo=None) == -1003 and fwd(z=None) == -1003
     bwd = lambda dx=p, part=p, dz=p, rx=p: lib.cpcsv_norm_residual_bwd(p, p, None, None, p, p, p, rx, p, dz, dx, p, None, None, p, p, part,
                                                                        4, 8, 0, 0, 0, 1, None)
     assert bwd(dx=None) == -1003 and bwd(part=None) == -1003 and bwd(rx=None) == -1003
