@@ -1489,14 +1489,13 @@ def _norm_forward(x, u, w_post, gate, scale, w_next, out_dtype, eps, keep):
     d = x.shape[-1]
     rows = x.numel() // d if d else 0
     dev, udt = x.device, dcode(u) if u is not None else (L.F32 if out_dtype == torch.float32 else L.BF16)
-    x = x.contiguous()
-    u, gate, w_post, scale, w_next = (None if q is None else q.contiguous() for q in (u, gate, w_post, scale, w_next))
+    x, u, gate, w_post, scale, w_next = (q if q is None or q.is_contiguous() else q.contiguous() for q in (x, u, gate, w_post, scale, w_next))
     mode, t = 0, 1
     if gate is not None:
         per = gate.numel() // d if d else 0
         mode, t = (1, 1) if per == rows else (2, rows // per)
-    xo = _empty(x.shape, x.dtype, dev) if u is not None else None
-    z = _empty(x.shape, out_dtype, dev) if w_next is not None else None
+    xo = _empty_like(x) if u is not None else None
+    z = (_empty_like(x) if out_dtype == x.dtype else _empty(x.shape, out_dtype, dev)) if w_next is not None else None
     ru = rx = None
     if rows:
         if keep:
@@ -1530,22 +1529,26 @@ class NormResidualFn(Function):
         if dxo is None and dz is None:
             return (None,) * 8
         need = ctx.needs_input_grad
-        dev, f32 = x.device, torch.float32
-        like = lambda q, on: _empty(q.shape, q.dtype, dev) if (on and q is not None) else None
-        dx, du, dgate = _empty(x.shape, x.dtype, dev), like(u, need[1]), like(gate, need[3])
-        dwp, dsc, dwn = like(w_post, need[2]), like(scale, need[4]), like(w_next, need[5])
+        dx = _empty_like(x)
+        du = _empty_like(u) if u is not None and need[1] else None
+        dwp = _empty_like(w_post) if w_post is not None and need[2] else None
+        dgate = _empty_like(gate) if gate is not None and need[3] else None
+        dsc = _empty_like(scale) if scale is not None and need[4] else None
+        dwn = _empty_like(w_next) if w_next is not None and need[5] else None
         if not rows:
             for q in (dwp, dsc, dwn, dgate):
                 if q is not None:
                     q.zero_()
             return dx, du, dwp, dgate, dsc, dwn, None, None
-        dxo = dxo.contiguous() if dxo is not None else None
-        dz = dz.contiguous() if dz is not None else None
+        if dxo is not None and not dxo.is_contiguous():
+            dxo = dxo.contiguous()
+        if dz is not None and not dz.is_contiguous():
+            dz = dz.contiguous()
         if dz is None and dwn is not None:
             dwn.zero_()
         part = None
         if dwp is not None or dsc is not None or dwn is not None or (mode == 2 and dgate is not None):
-            part = _empty((K.norm_residual_part(rows, d, mode, t),), f32, dev)
+            part = _empty((K.norm_residual_part(rows, d, mode, t),), torch.float32, x.device)
         K.norm_residual_bwd(x, u, gate, scale, w_post, w_next, ru, rx, dxo, dz, dx, du, dgate, dsc, dwp, dwn, part, rows, d, udt, mode, t)
         _runtime.keep_forced(dxo, dz, part)
         return dx, du, dwp, dgate, dsc, dwn, None, None
