@@ -190,18 +190,21 @@ __global__ __launch_bounds__(256) void orth_split_kernel(Jobs s) {
 }
 
 // ---- the products: D = alpha P Q^T + beta E + gamma I over two-plane operands [rows][K] ------------------------------
-enum { SYMM, BOTH, OUT };      // D symmetric: lower triangle and its mirror image | D and its transpose | the result or the weight
+// D symmetric, lower triangle and its mirror image (SYMM_E: with E and I) | D and its transpose | the result | the weight. A launch has
+// one kind and its own kernel: straight-line code for all of them was 68 KB, and what a block runs once comes cold from memory
+enum { SYMM, SYMM_E, BOTH, OUT, WEIGHT };
+__host__ __device__ constexpr bool symmetric(int kind) { return kind == SYMM || kind == SYMM_E; }
 struct Task {
-    long p, q, e, d, dt;       // offsets in halves (e < 0: none); OUT: d is the output's address
+    long p, q, e, d, dt;       // offsets in halves; OUT, WEIGHT: d is the output's address
     long slab;                 // first partial tile, in floats
     int R, C, K;
     float alpha, beta, gamma;
-    int kind, shape, t0, tiles, whole, S, r0; // tile shape; first block; tiles, of which `whole` in one piece, the others in S slices of K; first joining block
-    int rows, cols, tall;                     // OUT: of the output
+    int shape, t0, tiles, whole, S, r0; // tile shape; first block; tiles, of which `whole` in one piece, the others in S slices of K; first joining block
+    int rows, cols, tall;                     // OUT, WEIGHT: of the output
 };
 struct Launch {
     Task t[MAXT];
-    int n, dtype;
+    int n, kind, dtype;
     float decay;
     const float* hyper;
     _Float16* ws;
@@ -232,8 +235,8 @@ using Mid = Cfg<128, 64, 64, 32>;
 using Small = Cfg<64, 32, 32, 64>;
 static_assert(Big::LDS >= Big::NW * Big::STRIP * 4 && Mid::LDS >= Mid::NW * Mid::STRIP * 4 && Small::LDS >= Small::NW * Small::STRIP * 4, "strips fit");
 
-__device__ __forceinline__ void tile_of(const Task& t, int tile, int bm, int& ti, int& tj) {
-    if (t.kind == SYMM) {
+template <int KIND> __device__ __forceinline__ void tile_of(const Task& t, int tile, int bm, int& ti, int& tj) {
+    if (symmetric(KIND)) {
         // lower triangle by blocks of g x g tiles, a row of blocks behind the other (the last one of h tile rows; on the diagonal
         // triangles): a run of tiles shares operand rows in L2. Row by row, every XCD read the whole operand.
         const int n = (t.R + bm - 1) / bm, g = n >= 24 ? 8 : 4;
@@ -271,117 +274,99 @@ __device__ __forceinline__ uint32_t entry(const Launch& s, const Task& t, int r,
 }
 
 // One wavefront's strip, 32 rows x SW columns from (r0, c0), -> D. A lane's 16 values of a 32 x 32 block: column lane % 32, rows
-// 8 (i / 4) + 4 (lane / 32) + i % 4; they pass through the wavefront's own piece of LDS to leave as 16-byte pieces of rows in either
-// orientation.
-template <typename C, bool EARLY>
-__device__ __forceinline__ void finish(const Launch& s, const Task& t, int r0, int c0, const f32x16 (&acc)[C::NB], uint32_t* buf, const u32x16& early) {
-    constexpr int SW = C::SW, LDW = SW + 1, NB = C::NB;
+// 8 (i / 4) + 4 (lane / 32) + i % 4; they pass through the wavefront's own piece of LDS (to_lds) to leave as 16-byte pieces of rows in
+// either orientation (leave).
+template <typename C, int KIND, bool EARLY>
+__device__ __forceinline__ void to_lds(const Launch& s, const Task& t, int r0, int c0, const f32x16 (&acc)[C::NB], uint32_t* buf, const u32x16& early) {
     const int lane = threadIdx.x & 63, fr = lane & 31, fk = lane >> 5;
-    if (r0 >= t.R || c0 >= t.C || (t.kind == SYMM && r0 + 31 < c0)) return;                // (sides are multiples of a strip's)
-    const bool diag = t.kind == SYMM && r0 < c0 + SW;                                      // the strip meets the diagonal
-    const float lr = t.kind == OUT && s.hyper ? s.hyper[0] : 0.f;
-    const float keep = 1.f - lr * s.decay, step = lr * sqrtf(fmaxf(1.f, (float)t.rows / (float)t.cols));
-    asm volatile("" ::: "memory");               // (the next strip's loads are not hoisted over this one: they would not fit the registers)
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < C::NB; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int rl = (i >> 2) * 8 + fk * 4 + (i & 3), cl = b * 32 + fr, r = r0 + rl, c = c0 + cl;
             float v = acc[b][i] * t.alpha;
-            if (t.e >= 0) {
+            if (KIND == SYMM_E) {
                 union { uint32_t w; _Float16 h[2]; } p;
                 if (EARLY) p.w = early[i];                    // (one block a strip)
                 else p.w = entry(s, t, r, c);
                 v += ((float)p.h[0] + (float)p.h[1]) * t.beta + (r == c ? t.gamma : 0.f);
             }
-            buf[rl * LDW + cl] = t.kind == OUT ? __float_as_uint(v) : split_of(v);
+            buf[rl * (C::SW + 1) + cl] = KIND >= OUT ? __float_as_uint(v) : split_of(v);
         }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    if (t.kind == OUT) {
-        // rows of the output run along the strip's columns, of a tall one's along its rows
-        constexpr int GO = C::MA * C::MB > 4 ? 8 : SW / 2;
-        const int len = t.tall ? 32 : SW, per = 64 / len, sub = lane % len;
-#pragma unroll
-        for (int i0 = 0; i0 < SW / 2; i0 += GO) {
-            float old[GO];
-#pragma unroll
-            for (int i = 0; i < GO; ++i) {
-                const int l = (i0 + i) * per + lane / len, R = (t.tall ? c0 : r0) + l, Cc = (t.tall ? r0 : c0) + sub;
-                if (s.hyper && R < t.rows && Cc < t.cols) old[i] = ((float*)t.d)[(long)R * t.cols + Cc];
-            }
-#pragma unroll
-            for (int i = 0; i < GO; ++i) {
-                const int l = (i0 + i) * per + lane / len, R = (t.tall ? c0 : r0) + l, Cc = (t.tall ? r0 : c0) + sub;
-                const float v = __uint_as_float(t.tall ? buf[sub * LDW + l] : buf[l * LDW + sub]);
-                if (R >= t.rows || Cc >= t.cols) continue;
-                const long at = (long)R * t.cols + Cc;
-                if (s.hyper) ((float*)t.d)[at] = old[i] * keep - step * v;
-                else if (s.dtype == CPCSV_F32) ((float*)t.d)[at] = v;
-                else ((bf16_t*)t.d)[at] = f32_to_bf16(v);
-            }
-            asm volatile("" ::: "memory");       // (the big tile: eight at a time, all of them would not fit the registers)
-        }
-        return;
-    }
-    if (diag) {
-        // by 32 x 32 blocks: below the diagonal as elsewhere; on it, each pair of entries is taken from the lower one (the two sums
-        // are the same numbers in another order)
+}
+
+// a 32 x 32 block of the strip as rows of D from (r0, c0): itself, its transpose, or (on the diagonal) its lower triangle mirrored
+enum { SELF, TURNED, MIRRORED };
+template <typename C, int HOW> __device__ __forceinline__ void block_out(const uint32_t* z, _Float16* d, int r0, int c0, int K) {
+    const int lane = threadIdx.x & 63;
+    for (int i = 0; i < 2; ++i) {
+        const int line = i * 16 + lane / 4, q = lane % 4 * 8;
         uint32_t w[8];
         half8 hi, lo;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const int cb = c0 + b * 32;
-            if (cb > r0) continue;
+        for (int e = 0; e < 8; ++e)
+            w[e] = HOW == TURNED || (HOW == MIRRORED && line < q + e) ? z[(q + e) * (C::SW + 1) + line] : z[line * (C::SW + 1) + q + e];
+        planes_of(w, hi, lo);
+        _Float16* o = d + at_of(r0 + line, c0 + q, K);
+        *(half8*)o = hi;
+        *(half8*)(o + 32) = lo;
+    }
+}
+
+template <typename C, int KIND>
+__device__ __forceinline__ void leave(const Launch& s, const Task& t, int r0, int c0, const uint32_t* buf) {
+    constexpr int SW = C::SW, LDW = SW + 1, NB = C::NB;
+    const int lane = threadIdx.x & 63;
+    if (KIND >= OUT) {
+        // rows of the output run along the strip's columns, of a tall one's along its rows; GO rows at a time are read before they are
+        // written (the weight's: one after the other they cost a memory latency each)
+        constexpr int GO = 16;
+        const int len = t.tall ? 32 : SW, per = 64 / len, sub = lane % len, R0 = (t.tall ? c0 : r0) + lane / len, Cc = (t.tall ? r0 : c0) + sub;
+        const int sl = t.tall ? sub * LDW + lane / len : lane / len * LDW + sub, dl = t.tall ? per : per * LDW;
+        const long at0 = (long)R0 * t.cols + Cc, step = (long)per * t.cols;
+        const float lr = KIND == WEIGHT ? s.hyper[0] : 0.f;
+        const float keep = 1.f - lr * s.decay, by = lr * sqrtf(fmaxf(1.f, (float)t.rows / (float)t.cols));
+        const int n = Cc < t.cols && R0 < t.rows ? min(SW / 2, (t.rows - R0 + per - 1) / per) : 0;
+        typedef __attribute__((address_space(1))) float gf;
+        typedef __attribute__((address_space(1))) bf16_t gb;
+        for (int i0 = 0; i0 < n; i0 += GO) {
+            float old[GO];
+            if (KIND == WEIGHT)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int line = i * 16 + lane / 4, q = lane % 4 * 8;
-                const uint32_t* z = buf + b * 32;
+                for (int i = 0; i < GO; ++i) old[i] = ((gf*)t.d)[at0 + step * min(i0 + i, n - 1)];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) w[e] = cb == r0 && line < q + e ? z[(q + e) * LDW + line] : z[line * LDW + q + e];
-                planes_of(w, hi, lo);
-                _Float16* d = s.ws + t.d + at_of(r0 + line, cb + q, t.C);
-                *(half8*)d = hi;
-                *(half8*)(d + 32) = lo;
-                if (cb == r0) continue;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) w[e] = z[(q + e) * LDW + line];
-                planes_of(w, hi, lo);
-                d = s.ws + t.d + at_of(cb + line, r0 + q, t.C);
-                *(half8*)d = hi;
-                *(half8*)(d + 32) = lo;
+            for (int i = 0; i < GO; ++i) {
+                if (i0 + i >= n) continue;
+                const float v = __uint_as_float(buf[sl + dl * (i0 + i)]);
+                const long at = at0 + step * (i0 + i);
+                if (KIND == WEIGHT) ((gf*)t.d)[at] = old[i] * keep - by * v;
+                else if (s.dtype == CPCSV_F32) ((gf*)t.d)[at] = v;
+                else ((gb*)t.d)[at] = f32_to_bf16(v);
             }
         }
         return;
     }
-    uint32_t w[8];
-    half8 hi, lo;
-    constexpr int PC = SW / 8, RP = 64 / PC;              // 16-byte pieces of a strip row, rows a pass
-#pragma unroll
-    for (int i = 0; i < 32 / RP; ++i) {
-        const int rl = i * RP + lane / PC, cl = lane % PC * 8;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = buf[rl * LDW + cl + e];
-        planes_of(w, hi, lo);
-        _Float16* d = s.ws + t.d + at_of(r0 + rl, c0 + cl, t.C);
-        *(half8*)d = hi;
-        *(half8*)(d + 32) = lo;
-    }
-    _Float16* const turned = s.ws + (t.kind == SYMM ? t.d : t.dt);                 // (D^T [C][R]; R = C for a symmetric one)
-#pragma unroll
-    for (int i = 0; i < SW / 16; ++i) {
-        const int cl = i * 16 + lane / 4, rl = lane % 4 * 8;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = buf[(rl + e) * LDW + cl];
-        planes_of(w, hi, lo);
-        _Float16* d = turned + at_of(c0 + cl, r0 + rl, t.R);
-        *(half8*)d = hi;
-        *(half8*)(d + 32) = lo;
+    _Float16 *const d = s.ws + t.d, *const turned = s.ws + (symmetric(KIND) ? t.d : t.dt);             // (D^T [C][R])
+    for (int b = 0; b < NB; ++b) {
+        const int cb = c0 + b * 32;
+        if (symmetric(KIND) && cb > r0) continue;              // (above the diagonal)
+        if (symmetric(KIND) && cb == r0) {
+            // on it: each pair of entries is taken from the lower one (the two sums are the same numbers in another order)
+            block_out<C, MIRRORED>(buf + b * 32, d, r0, cb, t.C);
+            continue;
+        }
+        block_out<C, SELF>(buf + b * 32, d, r0, cb, t.C);
+        block_out<C, TURNED>(buf + b * 32, turned, cb, r0, t.R);
     }
 }
+
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+// (sides are multiples of a strip's)
+template <int KIND> __device__ __forceinline__ bool outside(const Task& t, int r0, int c0) { return r0 >= t.R || c0 >= t.C || (symmetric(KIND) && r0 + 31 < c0); }
 
 __device__ __forceinline__ const Task& task_of(const Launch& s) {
     if (s.n == 1) return s.t[0];
@@ -390,7 +375,7 @@ __device__ __forceinline__ const Task& task_of(const Launch& s) {
     return s.t[__popcll(__ballot(lane < s.n && (int)blockIdx.x >= first)) - 1];
 }
 
-template <typename C>
+template <typename C, int KIND>
 __device__ __forceinline__ void product(const Launch& s, const Task& t, unsigned char* smem) {
     _Float16* const lds = (_Float16*)smem;
     // the whole tiles first, then the others, slice by slice. Blocks go to the eight XCDs in turn: each gets a contiguous run of
@@ -401,7 +386,7 @@ __device__ __forceinline__ void product(const Launch& s, const Task& t, unsigned
     for (int x = 0; x < xcd; ++x) u += (n + 7 - ((x - from) & 7)) >> 3;
     const int S = sliced ? t.S : 1, sl = sliced ? u / cut : 0, tile = sliced ? t.whole + u % cut : u;
     int ti, tj;
-    tile_of(t, tile, C::BM, ti, tj);
+    tile_of<KIND>(t, tile, C::BM, ti, tj);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, K = t.K;
     const int nk = K / C::BK, k0 = (int)((long)nk * sl / S), k1 = (int)((long)nk * (sl + 1) / S);
     const _Float16* src[2] = {s.ws + t.p + (long)ti * C::BM * 2 * K, s.ws + t.q + (long)tj * C::BM * 2 * K};
@@ -436,7 +421,7 @@ __device__ __forceinline__ void product(const Launch& s, const Task& t, unsigned
     if (k0 < k1) stage(0, k0);
     constexpr bool ONE = C::MA * C::MB == 1;
     u32x16 early = {};
-    if (ONE && t.e >= 0 && S == 1) {
+    if (ONE && KIND == SYMM_E && S == 1) {
         const int r0 = ti * C::BM + wm, c0 = tj * C::BM + wn;
         if (r0 < t.R && c0 < t.C)
 #pragma unroll
@@ -494,33 +479,46 @@ __device__ __forceinline__ void product(const Launch& s, const Task& t, unsigned
                 }
         return;
     }
-    static_for<C::STRIPS>([&](auto i) {          // (a loop of this body is too long for the unroller, and its registers need constant indices)
-        constexpr int a = decltype(i)::value / (C::MB / C::NB), b = decltype(i)::value % (C::MB / C::NB) * C::NB;
-        f32x16 strip[C::NB];
+    uint32_t* const buf = (uint32_t*)smem + wave * C::STRIP;
+    for (int strip = 0; strip < C::STRIPS; ++strip) {
+        const int r0 = ti * C::BM + wm + strip / (C::MB / C::NB) * 32, c0 = tj * C::BM + wn + strip % (C::MB / C::NB) * C::NB * 32;
+        if (outside<KIND>(t, r0, c0)) continue;
+        static_for<C::STRIPS>([&](auto i) {      // (registers need constant indices)
+            if (i.value != strip) return;
+            constexpr int a = decltype(i)::value / (C::MB / C::NB), b = decltype(i)::value % (C::MB / C::NB) * C::NB;
+            f32x16 part[C::NB];
 #pragma unroll
-        for (int n = 0; n < C::NB; ++n) strip[n] = acc[a][b + n];
-        finish<C, ONE>(s, t, ti * C::BM + wm + a * 32, tj * C::BM + wn + b * 32, strip, (uint32_t*)smem + wave * C::STRIP, early);
-    });
+            for (int n = 0; n < C::NB; ++n) part[n] = acc[a][b + n];
+            to_lds<C, KIND, ONE>(s, t, r0, c0, part, buf, early);
+        });
+        wave_sync();
+        leave<C, KIND>(s, t, r0, c0, buf);
+        wave_sync();
+    }
 }
 
 // one launch serves the two shapes of 256 threads and 64 KB of LDS
+template <int KIND>
 __global__ __launch_bounds__(Mid::T) void orth_gemm_kernel(Launch s) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const Task& t = task_of(s);
-    if (t.shape == 1) product<Mid>(s, t, smem);
-    else product<Small>(s, t, smem);
+    if (t.shape == 1) product<Mid, KIND>(s, t, smem);
+    else product<Small, KIND>(s, t, smem);
 }
+template <int KIND>
 __global__ __launch_bounds__(Big::T) void orth_gemm_big_kernel(Launch s) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    product<Big>(s, task_of(s), smem);
+    product<Big, KIND>(s, task_of(s), smem);
 }
 
 // the slices of a tile, added in order: one wavefront a strip
-template <typename C> __device__ __forceinline__ void join(const Launch& s, const Task& t, uint32_t* buf) {
+template <typename C, int KIND> __device__ __forceinline__ void join(const Launch& s, const Task& t, uint32_t* buf) {
     const int id = blockIdx.x - t.r0, strip = id % (C::NW * C::STRIPS), cut = id / (C::NW * C::STRIPS), wave = strip / C::STRIPS;
     const int a = strip % C::STRIPS / (C::MB / C::NB), b = strip % (C::MB / C::NB) * C::NB;
     int ti, tj;
-    tile_of(t, t.whole + cut, C::BM, ti, tj);
+    tile_of<KIND>(t, t.whole + cut, C::BM, ti, tj);
+    const int r0 = ti * C::BM + wave / C::WC * C::WM + a * 32, c0 = tj * C::BM + wave % C::WC * C::WN + b * 32;
+    if (outside<KIND>(t, r0, c0)) return;
     const f32x4* d = (const f32x4*)(s.slabs + t.slab) + (long)cut * t.S * (C::BM * C::BM / 4) + (long)strip * C::NB * 256 + threadIdx.x;
     f32x16 acc[C::NB];
 #pragma unroll
@@ -537,22 +535,25 @@ template <typename C> __device__ __forceinline__ void join(const Launch& s, cons
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[n][h * 4 + e] += v[e];
             }
-    finish<C, false>(s, t, ti * C::BM + wave / C::WC * C::WM + a * 32, tj * C::BM + wave % C::WC * C::WN + b * 32, acc, buf, u32x16{});
+    to_lds<C, KIND, false>(s, t, r0, c0, acc, buf, u32x16{});
+    wave_sync();
+    leave<C, KIND>(s, t, r0, c0, buf);
 }
+template <int KIND>
 __global__ __launch_bounds__(64) void orth_join_kernel(Launch s) {
     __shared__ uint32_t buf[Mid::STRIP];
     const int first = s.t[min((int)threadIdx.x, s.n - 1)].r0;
     const Task& t = s.t[__popcll(__ballot((int)threadIdx.x < s.n && (int)blockIdx.x >= first)) - 1];
-    if (t.shape == 0) join<Big>(s, t, buf);
-    else if (t.shape == 1) join<Mid>(s, t, buf);
-    else join<Small>(s, t, buf);
+    if (t.shape == 0) join<Big, KIND>(s, t, buf);
+    else if (t.shape == 1) join<Mid, KIND>(s, t, buf);
+    else join<Small, KIND>(s, t, buf);
 }
 static_assert(Mid::T == Small::T && Mid::LDS == Small::LDS && Mid::STRIP >= Small::STRIP && Mid::STRIP >= Big::STRIP, "shared launches");
 
 // ---- host: the schedule ---------------------------------------------------------------------------------------------
 long tiles_of(int kind, long R, long C, int bm) {
     const long tm = (R + bm - 1) / bm, tn = (C + bm - 1) / bm;
-    return kind == SYMM ? tm * (tm + 1) / 2 : tm * tn;
+    return symmetric(kind) ? tm * (tm + 1) / 2 : tm * tn;
 }
 // How a product is cut: the tile, and how many slices of K the tiles get that do not fill the last round of blocks over the 256 CUs
 // (all of them, where there are few: 1024 x 18432 against itself has 36 of 128 x 128 and took 470 us in one piece). By the
@@ -618,6 +619,17 @@ int plan(Jobs& s, Scratch* sc, const long* dims, int njobs, Plan& p) {
     return 0;
 }
 
+template <int KIND> int fire(const Launch& big, const Launch& rest, const Launch& join, long ubig, long urest, long joins, hipStream_t st) {
+    if (big.n) {                                                // more than the default cap of dynamic LDS: raise it once
+        static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(orth_gemm_big_kernel<KIND>), hipFuncAttributeMaxDynamicSharedMemorySize, Big::LDS);
+        if (e != hipSuccess) return -(int)e;
+        orth_gemm_big_kernel<KIND><<<(int)ubig, Big::T, Big::LDS, st>>>(big);
+    }
+    if (rest.n) orth_gemm_kernel<KIND><<<(int)urest, Mid::T, Mid::LDS, st>>>(rest);
+    if (join.n) orth_join_kernel<KIND><<<(int)joins, 64, 0, st>>>(join);
+    CPCSV_CHECK_LAUNCH();
+    return 0;
+}
 // the products of one level: a launch for those of the big tile, one for the others, one that joins slices
 int run_level(const Launch& all, long slabs, hipStream_t st) {
     Launch big = all, rest = all, join = all;
@@ -625,9 +637,9 @@ int run_level(const Launch& all, long slabs, hipStream_t st) {
     long at = 0, units[2] = {0, 0}, joins = 0;
     for (int i = 0; i < all.n; ++i) {
         Task t = all.t[i];
-        const Cut cut = cut_of(t.kind, t.R, t.C, t.K);
+        const Cut cut = cut_of(all.kind, t.R, t.C, t.K);
         t.shape = cut.shape;
-        t.tiles = (int)tiles_of(t.kind, t.R, t.C, SHAPES[cut.shape].bm);
+        t.tiles = (int)tiles_of(all.kind, t.R, t.C, SHAPES[cut.shape].bm);
         t.whole = cut.whole; t.S = cut.S; t.slab = at;
         at += cut.slab;
         long& u = units[cut.shape != 0];
@@ -640,15 +652,13 @@ int run_level(const Launch& all, long slabs, hipStream_t st) {
         if (t.S > 1) join.t[join.n++] = t;
     }
     if (at > slabs) return -1004;
-    if (big.n) {                                                // more than the default cap of dynamic LDS: raise it once
-        static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(orth_gemm_big_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, Big::LDS);
-        if (e != hipSuccess) return -(int)e;
-        orth_gemm_big_kernel<<<(int)units[0], Big::T, Big::LDS, st>>>(big);
+    switch (all.kind) {
+        case SYMM: return fire<SYMM>(big, rest, join, units[0], units[1], joins, st);
+        case SYMM_E: return fire<SYMM_E>(big, rest, join, units[0], units[1], joins, st);
+        case BOTH: return fire<BOTH>(big, rest, join, units[0], units[1], joins, st);
+        case OUT: return fire<OUT>(big, rest, join, units[0], units[1], joins, st);
+        default: return fire<WEIGHT>(big, rest, join, units[0], units[1], joins, st);
     }
-    if (rest.n) orth_gemm_kernel<<<(int)units[1], Mid::T, Mid::LDS, st>>>(rest);
-    if (join.n) orth_join_kernel<<<(int)joins, 64, 0, st>>>(join);
-    CPCSV_CHECK_LAUNCH();
-    return 0;
 }
 
 int iterate(Jobs& s, const Scratch* sc, const Plan& p, int steps, const float* hyper, float decay, void* ws, hipStream_t st) {
@@ -662,7 +672,8 @@ int iterate(Jobs& s, const Scratch* sc, const Plan& p, int steps, const float* h
     auto add = [&](int kind, const Job& j, long pp, long q, long d, int C, int K, float alpha) -> Task& {
         Task& t = L.t[L.n++];
         t = Task{};
-        t.p = pp; t.q = q; t.d = d; t.e = -1; t.R = j.M; t.C = C; t.K = K; t.alpha = alpha; t.kind = kind;
+        t.p = pp; t.q = q; t.d = d; t.R = j.M; t.C = C; t.K = K; t.alpha = alpha;
+        L.kind = kind;
         return t;
     };
     auto level = [&]() { const int rc = run_level(L, p.slabs, st); L.n = 0; return rc; };
@@ -677,7 +688,7 @@ int iterate(Jobs& s, const Scratch* sc, const Plan& p, int steps, const float* h
         LEVEL(add(SYMM, j, j.x, j.x, c.a, j.M, j.N, SA / (SX * SX)););
         for (int k = 1; k <= run; ++k) {
             // P_k in p0, p1 in turn; Q_1 = P_1, Q_2 = P_2 P_1 in q0, Q_3 = P_3 Q_2 in q1
-            LEVEL(Task& t = add(SYMM, j, c.a, c.a, k & 1 ? c.p0 : c.p1, j.M, j.M, NS_C * SP / (SA * SA));
+            LEVEL(Task& t = add(SYMM_E, j, c.a, c.a, k & 1 ? c.p0 : c.p1, j.M, j.M, NS_C * SP / (SA * SA));
                   t.e = c.a; t.beta = NS_B * SP / SA; t.gamma = NS_A * SP;);
             if (k > 1 || k < run)
                 LEVEL(const long pk = k & 1 ? c.p0 : c.p1;
@@ -687,7 +698,7 @@ int iterate(Jobs& s, const Scratch* sc, const Plan& p, int steps, const float* h
         }
         done += run;
         LEVEL(const long q = run == 1 ? c.p0 : run == 2 ? c.q0 : c.q1;
-              Task& t = add(done < steps ? BOTH : OUT, j, q, odd ? c.xt1 : j.xt, j.x, j.N, j.M, 1.f / SQ[run]);
+              Task& t = add(done < steps ? BOTH : hyper ? WEIGHT : OUT, j, q, odd ? c.xt1 : j.xt, j.x, j.N, j.M, 1.f / SQ[run]);
               if (done < steps) t.dt = odd ? j.xt : c.xt1;
               else { t.d = (long)j.out; t.alpha /= SX; t.rows = j.rows; t.cols = j.cols; t.tall = j.tall; });
         odd = !odd;
