@@ -1477,6 +1477,8 @@ def gated_scan_step(p, h, out_gate=True):
     y = _empty((b, hid), p.dtype, p.device)
     if b:
         K.scan_step(p, h, y, b, hid, out_gate)
+        if not h.is_inference():
+            torch.autograd.graph.increment_version(h)      # (a graph that saved this state refuses its backward pass)
         _runtime.keep_forced(p)
     return y
 
@@ -1561,6 +1563,8 @@ def _norm_call(*args):
 
 
 def _norm_vec(name, w, d):
+    if w is None:
+        raise TypeError("%s must be given" % name)
     if w.dtype != torch.float32:
         raise TypeError("%s must be float32, got %s" % (name, w.dtype))
     if w.shape != (d,):
@@ -1601,7 +1605,7 @@ def norm_residual(x, u, w_post, gate=None, scale=None, w_next=None, eps=1e-6):
     if u.shape != x.shape:
         raise ValueError("u must have x's shape %s, got %s" % (tuple(x.shape), tuple(u.shape)))
     for name, w in (("w_post", w_post), ("scale", scale), ("w_next", w_next)):
-        if w is not None:
+        if w is not None or name == "w_post":
             _norm_vec(name, w, d)
     if gate is not None:
         if gate.dtype != u.dtype:

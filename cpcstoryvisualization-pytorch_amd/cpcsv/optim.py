@@ -327,6 +327,10 @@ class FusedMuon(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=int(steps), eps=eps))
         self._hypers = {}
 
+    def __setstate__(self, state):               # (copies and unpickled optimisers; load_state_dict comes here too and keeps the scalars)
+        super().__setstate__(state)
+        self.__dict__.setdefault("_hypers", {})
+
     def add_param_group(self, group):
         super().add_param_group(group)
         for p in self.param_groups[-1]["params"]:
@@ -372,6 +376,8 @@ class FusedMuon(torch.optim.Optimizer):
                 if not ok(p) or not ok(p.grad):
                     raise RuntimeError("FusedMuon needs contiguous fp32 GPU parameters and gradients")
                 if "momentum_buffer" not in st:
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("FusedMuon: a parameter without momentum during capture (each replay would begin it anew): run one step with it before")
                     st["momentum_buffer"] = torch.zeros_like(p)
                 elif not ok(st["momentum_buffer"]):
                     raise RuntimeError("FusedMuon needs contiguous fp32 GPU momentum of the parameter's shape")

@@ -348,7 +348,8 @@ int tpr_of(int D, int per) {                // threads a row: the fewest wavefro
 }
 int check(const NormArgs& a, int xdt, int udt, int gmode) {
     if (!((xdt == CPCSV_F32 || xdt == CPCSV_BF16) && (udt == CPCSV_F32 || udt == CPCSV_BF16)) || (xdt == CPCSV_BF16 && udt == CPCSV_F32)) return -1001;
-    if (a.rows <= 0 || a.D <= 0 || a.D > CPCSV_NORM_MAX_D || gmode < 0 || gmode > 2 || (gmode == 2 && (a.T <= 0 || a.rows % a.T))) return -1002;
+    if (a.rows <= 0 || a.D <= 0 || a.D > CPCSV_NORM_MAX_D || gmode < 0 || gmode > 2 || (gmode == 2 && (a.T <= 0 || a.rows % a.T || a.rows / a.T > (1L << 30))))
+        return -1002;
     if (!a.x || (a.u && !a.w_post) || (gmode && (!a.gate || !a.u)) || (!a.u && !a.w_next)) return -1003;
     return 0;
 }

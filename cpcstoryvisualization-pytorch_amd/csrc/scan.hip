@@ -462,7 +462,9 @@ bool pairs_ok(int dtype, int H, long sb, long st, const void* a, const void* b, 
 int dims_of(Dims& d, int dtype, int B, int T, int H, long sb, long st, const int* len, int vec) {
     if ((dtype != CPCSV_F32 && dtype != CPCSV_BF16) || B <= 0 || T <= 0 || H <= 0 || T > CPCSV_SCAN_MAX_T) return -1001;
     d = Dims{B, T, H, H / vec, 0, (T + CH - 1) / CH, sb, st, len};
-    if ((long)tiles_of(T, BW) * B * ((d.G + 63) / 64) > (1L << 30) || (long)B * d.G > (1L << 38)) return -1002;
+    // a launch holds fewer than 2^32 threads
+    const long groups = (d.G + 63L) / 64, threads = T <= SHORT ? (long)B * d.G : max((long)tiles_of(T, FW) * FW, (long)tiles_of(T, BW) * BW) * 64;
+    if (threads >= (1L << 32) - TB || (T > SHORT && threads * B >= (1L << 32) / groups)) return -1002;
     return 0;
 }
 }  // namespace

@@ -16,6 +16,8 @@ def test_norm_residual_refuses():
         F.norm_residual(x, x[:1], w)
     with pytest.raises(TypeError, match="w_post must be float32"):
         F.norm_residual(x, x, w.bfloat16())
+    with pytest.raises(TypeError, match="w_post must be given"):
+        F.norm_residual(x, x, None)
     for bad in (dict(w_post=torch.ones(7)), dict(w_post=w, scale=torch.ones(1)), dict(w_post=w, w_next=torch.ones(1, 8))):
         with pytest.raises(ValueError, match="must have shape"):
             F.norm_residual(x, x, **bad)
@@ -60,6 +62,7 @@ def test_entry_points_reject_bad_arguments():
         x, u, gate, None, wp, wn, xo, z, p, p, rows, d, xdt, udt, mode, t, 1e-6, None)
     assert fwd(xdt=1, udt=0) == -1001 and fwd(udt=5) == -1001
     assert fwd(rows=0) == -1002 and fwd(d=0) == -1002 and fwd(d=16385) == -1002 and fwd(mode=3) == -1002
+    assert fwd(mode=2, gate=p, rows=(1 << 30) + 1) == -1002
     assert fwd(mode=2, gate=p, t=3) == -1002 and fwd(mode=2, gate=p, t=0) == -1002
     assert fwd(x=None) == -1003 and fwd(wp=None) == -1003 and fwd(mode=1) == -1003 and fwd(u=None, wn=None) == -1003 and fwd(xo=None) == -1003 and fwd(z=None) == -1003
     bwd = lambda dx=p, part=p, dz=p, rx=p: lib.cpcsv_norm_residual_bwd(p, p, None, None, p, p, p, rx, p, dz, dx, p, None, None, p, p, part,

@@ -254,3 +254,85 @@ def test_muon_refuses_on_the_gpu():
     opt.state[p]["momentum_buffer"] = torch.zeros(6, 4).cuda()
     with pytest.raises(RuntimeError, match="momentum"):
         opt.step()
+    q = torch.nn.Parameter(torch.zeros(4, 6).cuda())
+    late = FusedMuon([torch.nn.Parameter(torch.zeros(4, 6).cuda()), q])
+    late.param_groups[0]["params"][0].grad = torch.zeros(4, 6).cuda()
+    late.step()
+    q.grad = torch.ones_like(q)
+    with pytest.MonkeyPatch.context() as m:                  # (its first gradient arrives while a step is captured)
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="without momentum during capture"):
+            late.step()
+        with pytest.raises(RuntimeError, match="run one step before"):
+            other = FusedMuon([q])
+            other.state[q]["momentum_buffer"] = torch.zeros_like(q)
+            other.step()
+    late.step()
+    assert not torch.equal(q, torch.zeros_like(q))
+
+
+# padded sides by what they reach: whole and sliced tiles of the three shapes, both orientations
+LARGE = [(2049, 2050), (1600, 5200), (6400, 2816), (900, 16300), (2304, 5376), (4990, 5000), (5700, 5760)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols", LARGE)
+def test_large_matrices(rows, cols, dtype):
+    from cpcsv.optim import orthogonalize
+    g = torch.randn(rows, cols, generator=torch.Generator("cuda").manual_seed(rows), device="cuda").to(dtype)
+    got, want = orthogonalize(g), iterate(g, 5, 1e-7)
+    err, scale = (got.double() - want).norm().item(), want.norm().item()
+    assert err <= (bound(g.shape) + torch.finfo(dtype).eps / 2) * scale, err / scale
+    if dtype == torch.float32:
+        own = (iterate(g, 5, 1e-7, torch.float32).double() - want).norm().item()
+        assert err <= 4 * own + 2.0 ** -22 * scale, (err, own)
+    assert torch.equal(got, orthogonalize(g))
+
+
+@pytest.mark.parametrize("rows,cols", [(5200, 1600), (6400, 2816), (900, 16300), (2049, 2050)])
+def test_muon_large_matrices(rows, cols):
+    """The weight is updated in the tail of the last products: tall, wide, joined from slices; a small matrix beside it."""
+    from cpcsv.optim import FusedMuon
+    gen = torch.Generator("cuda").manual_seed(cols)
+    ps = [torch.nn.Parameter(0.05 * torch.randn(s, generator=gen, device="cuda")) for s in ((rows, cols), (70, 90))]
+    opt = FusedMuon(ps, lr=0.02, momentum=0.9, weight_decay=0.1)
+    want = []
+    for p in ps:
+        p.grad = torch.randn(p.shape, generator=gen, device="cuda")
+        w, _, size = step64(p.detach(), p.grad, torch.zeros_like(p), 0.02, 0.9, True, 0.1)
+        want.append((w, bound(p.shape) * size + 3 * 2.0 ** -24 * w.norm().item()))
+    opt.step()
+    for p, (w, tol) in zip(ps, want):
+        assert (p.detach().double() - w).norm().item() <= tol, tuple(p.shape)
+
+
+def test_copies_of_the_optimiser_continue():
+    import pickle
+    from cpcsv.optim import FusedMuon
+    p = torch.nn.Parameter(torch.eye(8, 12).cuda())
+    p.grad = torch.ones_like(p)
+    opt = FusedMuon([p], lr=0.1)
+    opt.step()
+    twins = [copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))]
+    opt.step()
+    for t in twins:
+        q = t.param_groups[0]["params"][0]
+        q.grad = torch.ones_like(q)
+        t.step()
+        assert torch.equal(q, p)
+
+
+def test_two_calls_at_once():
+    from cpcsv.optim import orthogonalize
+    gs = [spectrum(600, 900, "gauss", i).cuda() for i in (7, 8)]
+    want = [orthogonalize(g) for g in gs]
+    streams = [torch.cuda.Stream() for _ in gs]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for g, s in zip(gs, streams):
+            with torch.cuda.stream(s):
+                got.append(orthogonalize(g))
+    torch.cuda.synchronize()
+    for i, x in enumerate(got):
+        assert torch.equal(x, want[i % 2]), i

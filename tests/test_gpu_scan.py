@@ -317,3 +317,36 @@ def test_long_offsets(t):
     y, last = F.gated_scan(view, h0.cuda())
     y2, last2 = F.gated_scan(p.cuda(), h0.cuda())
     assert torch.equal(y, y2) and torch.equal(last, last2)
+
+
+@pytest.mark.parametrize("t", [20, 100])
+def test_a_state_updated_in_place_is_not_used_backward(t):
+    """gated_scan keeps its initial state for the backward pass: stepping that very tensor on is noticed."""
+    from cpcsv import functional as F
+    p, h0, dy, _, _ = make(2, t, 8, True, torch.float32, seed=8)
+    p, h = p.cuda().requires_grad_(), h0.cuda()
+    y, _ = F.gated_scan(p, h)
+    F.gated_scan_step(p.detach()[:, 0].contiguous(), h)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(dy.cuda())
+    with torch.inference_mode():
+        q, g = p.detach()[:, 0].clone(), h.clone()
+        F.gated_scan_step(q, g)
+    assert not torch.equal(g, h)
+
+
+def test_two_calls_at_once():
+    """Two streams, more blocks than the chip holds: each call waits for its own blocks only."""
+    cases = [[q.cuda() if q is not None else None for q in make(3, 3000, 512, True, torch.bfloat16, seed=s)] for s in (9, 10)]
+    want = [run(*[q.detach() if q is not None else None for q in c], True) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        for c, s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                got.append(run(*[q.detach() if q is not None else None for q in c], True))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        for k in g:
+            assert torch.equal(g[k], want[i % 2][k]), (i, k)

@@ -61,3 +61,13 @@ def test_scan_entry_points_reject_bad_arguments():
     assert fwd(p=None) == -1003 and fwd(y=None) == -1003 and fwd(T=64) == -1003 and fwd(T=64, ws=odd) == -1003
     bwd = lambda hin=one, dy=one, dp=one, ws=one, T=64: lib.cpcsv_scan_bwd(one, 0, 1, 1, None, None, hin, dy, None, dp, None, ws, 1, T, 1, 1, None)
     assert bwd(hin=None) == -1003 and bwd(ws=None) == -1003 and bwd(ws=odd) == -1003 and bwd(dy=None) == -1003 and bwd(dp=None, T=1) == -1003
+
+
+def test_launches_beyond_the_grid_are_refused():
+    """(2^32 threads a launch: refused before anything is started, whatever the runtime would do with them)"""
+    from cpcsv import _lib
+    lib = _lib.load()
+    one = 0x1000
+    for B, T, H in ((1 << 30, 1, 8), (1 << 22, 32, 1024), (1 << 24, 33, 1), (16, 1 << 28, 1), (1, 1 << 28, 1024)):
+        assert lib.cpcsv_scan_fwd(one, 0, 1, 1, None, None, one, None, None, one, B, T, H, 1, None) == -1002, (B, T, H)
+        assert lib.cpcsv_scan_bwd(one, 0, 1, 1, None, None, one, one, None, one, None, one, B, T, H, 1, None) == -1002, (B, T, H)
