@@ -24,8 +24,8 @@
 
 namespace {
 typedef __attribute__((ext_vector_type(8))) _Float16 half8;
+typedef __attribute__((ext_vector_type(4))) _Float16 half4;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
-typedef __attribute__((ext_vector_type(16))) uint32_t u32x16;
 
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 // Entries are bounded by spectral norms: |X| < 1.21, |A| and |P A| < 1.45, |P| < 3.45, |Q| < 3.45^k behind k iterations. The scaled
@@ -217,22 +217,22 @@ struct Launch {
 // Small products are bound by the latency of their K steps and of what stands before and behind them: 64 x 64 tiles, whose single
 // block a wavefront keeps two accumulators (a chain of dependent MFMAs half as long) and has its entries of E loaded beforehand
 // (512^3: 6.7 us for the bare product against 13.3 and 34).
-template <int BM_, int WM_, int WN_, int BK_> struct Cfg {
-    static constexpr int BM = BM_, WM = WM_, WN = WN_, BK = BK_, WC = BM / WN, NW = (BM / WM) * WC, T = NW * 64;
+template <int BM_, int WM_, int WN_, int RING_> struct Cfg {
+    static constexpr int BM = BM_, WM = WM_, WN = WN_, BK = 32, RING = RING_, WC = BM / WN, NW = (BM / WM) * WC, T = NW * 64;
     static constexpr int CPR = BK / 4;                            // 16-byte chunks of a row's slice, both halves
     static constexpr int LD = BM * CPR / T;                       // loads a thread, operand and stage
     static constexpr int STAGE = 4 * BM * BK;                     // halves
     static constexpr int SW = WN < 64 ? WN : 64, NB = SW / 32;    // columns of an epilogue strip, their 32 x 32 blocks
     static constexpr int STRIP = 32 * (SW + 1);                   // words of a strip in LDS
-    static constexpr int LDS = 2 * STAGE * 2;                     // (rings of 3 and 4 stages were no faster, and cost the second block on a CU)
+    static constexpr int LDS = RING * STAGE * 2;
     static constexpr int MA = WM / 32, MB = WN / 32, STRIPS = MA * MB / NB;
     // chunk (16 bytes) q of LDS row r lives in slot q ^ swz(r): the rows a fragment read touches together fall into all banks. The
     // DMA writes LDS in lane order, so the permutation is on the source side.
-    static __device__ __forceinline__ int swz(int r) { return CPR == 8 ? (r >> 1) & 7 : r & 15; }
+    static __device__ __forceinline__ int swz(int r) { return (r >> 1) & 7; }
 };
-using Big = Cfg<256, 128, 64, 32>;
-using Mid = Cfg<128, 64, 64, 32>;
-using Small = Cfg<64, 32, 32, 64>;
+using Big = Cfg<256, 128, 64, 2>;
+using Mid = Cfg<128, 64, 64, 2>;
+using Small = Cfg<64, 32, 32, 4>;
 static_assert(Big::LDS >= Big::NW * Big::STRIP * 4 && Mid::LDS >= Mid::NW * Mid::STRIP * 4 && Small::LDS >= Small::NW * Small::STRIP * 4, "strips fit");
 
 template <int KIND> __device__ __forceinline__ void tile_of(const Task& t, int tile, int bm, int& ti, int& tj) {
@@ -265,33 +265,32 @@ template <int N, typename F> __device__ __forceinline__ void static_for(F&& f) {
     }
 }
 
-__device__ __forceinline__ uint32_t entry(const Launch& s, const Task& t, int r, int c) {               // of E, hi | lo << 16
-    union { uint32_t w; _Float16 h[2]; } p;
-    const _Float16* o = s.ws + t.e + at_of(r, c, t.C);
-    p.h[0] = o[0];
-    p.h[1] = o[32];
-    return p.w;
+// E (symmetric, bit for bit) in rows r..r + 3 of column c, r a multiple of 4: read along row c, hi and lo
+struct Quad { half4 hi, lo; };
+__device__ __forceinline__ Quad quad_of(const Launch& s, const Task& t, int r, int c) {
+    const _Float16* o = s.ws + t.e + at_of(c, r, t.C);
+    return Quad{*(const half4*)o, *(const half4*)(o + 32)};
 }
 
 // One wavefront's strip, 32 rows x SW columns from (r0, c0), -> D. A lane's 16 values of a 32 x 32 block: column lane % 32, rows
 // 8 (i / 4) + 4 (lane / 32) + i % 4; they pass through the wavefront's own piece of LDS (to_lds) to leave as 16-byte pieces of rows in
 // either orientation (leave).
 template <typename C, int KIND, bool EARLY>
-__device__ __forceinline__ void to_lds(const Launch& s, const Task& t, int r0, int c0, const f32x16 (&acc)[C::NB], uint32_t* buf, const u32x16& early) {
+__device__ __forceinline__ void to_lds(const Launch& s, const Task& t, int r0, int c0, const f32x16 (&acc)[C::NB], uint32_t* buf, const Quad (&early)[4]) {
     const int lane = threadIdx.x & 63, fr = lane & 31, fk = lane >> 5;
 #pragma unroll
     for (int b = 0; b < C::NB; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int rl = (i >> 2) * 8 + fk * 4 + (i & 3), cl = b * 32 + fr, r = r0 + rl, c = c0 + cl;
-            float v = acc[b][i] * t.alpha;
-            if (KIND == SYMM_E) {
-                union { uint32_t w; _Float16 h[2]; } p;
-                if (EARLY) p.w = early[i];                    // (one block a strip)
-                else p.w = entry(s, t, r, c);
-                v += ((float)p.h[0] + (float)p.h[1]) * t.beta + (r == c ? t.gamma : 0.f);
+        for (int g = 0; g < 4; ++g) {
+            const int rl = g * 8 + fk * 4, cl = b * 32 + fr, r = r0 + rl, c = c0 + cl;
+            Quad q{};
+            if (KIND == SYMM_E) q = EARLY ? early[g] : quad_of(s, t, r, c);      // (early: one block a strip)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float v = acc[b][g * 4 + j] * t.alpha;
+                if (KIND == SYMM_E) v += ((float)q.hi[j] + (float)q.lo[j]) * t.beta + (r + j == c ? t.gamma : 0.f);
+                buf[(rl + j) * (C::SW + 1) + cl] = KIND >= OUT ? __float_as_uint(v) : split_of(v);
             }
-            buf[rl * (C::SW + 1) + cl] = KIND >= OUT ? __float_as_uint(v) : split_of(v);
         }
 }
 
@@ -368,6 +367,9 @@ __device__ __forceinline__ void wave_sync() {
 // (sides are multiples of a strip's)
 template <int KIND> __device__ __forceinline__ bool outside(const Task& t, int r0, int c0) { return r0 >= t.R || c0 >= t.C || (symmetric(KIND) && r0 + 31 < c0); }
 
+// all but the N youngest loads have landed, the wavefront's LDS reads are done
+template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
+
 __device__ __forceinline__ const Task& task_of(const Launch& s) {
     if (s.n == 1) return s.t[0];
     // (all first blocks compared at once: a search would be a chain of dependent loads)
@@ -387,26 +389,28 @@ __device__ __forceinline__ void product(const Launch& s, const Task& t, unsigned
     const int S = sliced ? t.S : 1, sl = sliced ? u / cut : 0, tile = sliced ? t.whole + u % cut : u;
     int ti, tj;
     tile_of<KIND>(t, tile, C::BM, ti, tj);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, K = t.K;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), K = t.K;
     const int nk = K / C::BK, k0 = (int)((long)nk * sl / S), k1 = (int)((long)nk * (sl + 1) / S);
     const _Float16* src[2] = {s.ws + t.p + (long)ti * C::BM * 2 * K, s.ws + t.q + (long)tj * C::BM * 2 * K};
-    int off[2][C::LD];                           // (K <= 131072 and 256 rows: below 2^31)
+    uint32_t off[2][C::LD];                      // in bytes (K <= 131072 and 256 rows: below 2^28)
 #pragma unroll
     for (int o = 0; o < 2; ++o)
 #pragma unroll
         for (int i = 0; i < C::LD; ++i) {
             const int idx = i * C::T + tid, row = idx / C::CPR, q = (idx % C::CPR) ^ C::swz(row);
             const int last = (o ? t.C - tj * C::BM : t.R - ti * C::BM) - 1;               // a tile may hang over the padded side
-            off[o][i] = min(row, last) * 2 * K + q * 8;
+            off[o][i] = (uint32_t)(min(row, last) * 2 * K + q * 8) * 2;
         }
+    auto load = [&](int buf, int kt, int o, int i) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)((const char*)(src[o] + (long)kt * 2 * C::BK) + off[o][i]),
+                                         (__attribute__((address_space(3))) void*)(lds + buf * C::STAGE + o * C::BM * 2 * C::BK +
+                                                                                   (i * C::T + wave * 64) * 8), 16, 0, 0);
+    };
     auto stage = [&](int buf, int kt) {
 #pragma unroll
         for (int o = 0; o < 2; ++o)
 #pragma unroll
-            for (int i = 0; i < C::LD; ++i)
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[o] + off[o][i] + (long)kt * 2 * C::BK),
-                                                 (__attribute__((address_space(3))) void*)(lds + buf * C::STAGE + o * C::BM * 2 * C::BK +
-                                                                                           (i * C::T + wave * 64) * 8), 16, 0, 0);
+            for (int i = 0; i < C::LD; ++i) load(buf, kt, o, i);
     };
     const int wm = wave / C::WC * C::WM, wn = wave % C::WC * C::WN, fr = lane & 31, fk = lane >> 5;
     f32x16 acc[C::MA][C::MB], low;               // low: the hi lo terms of a one-block wavefront
@@ -420,48 +424,85 @@ __device__ __forceinline__ void product(const Launch& s, const Task& t, unsigned
     }
     if (k0 < k1) stage(0, k0);
     constexpr bool ONE = C::MA * C::MB == 1;
-    u32x16 early = {};
+    Quad early[4] = {};
     if (ONE && KIND == SYMM_E && S == 1) {
         const int r0 = ti * C::BM + wm, c0 = tj * C::BM + wn;
         if (r0 < t.R && c0 < t.C)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) early[i] = entry(s, t, r0 + (i >> 2) * 8 + fk * 4 + (i & 3), c0 + fr);
+            for (int g = 0; g < 4; ++g) early[g] = quad_of(s, t, r0 + g * 8 + fk * 4, c0 + fr);
     }
+    if constexpr (ONE) {
+        // One wavefront a SIMD: what bounds a step is what it has to issue. Unrolled over the ring, so that LDS addresses are constants;
+        // all fragments first, the loads between the MFMAs; the RING - 1 stages in flight are behind a barrier of its own (one with
+        // the compiler's fence would wait for them).
+        constexpr int KK = C::BK / 16, EACH = 2 * C::LD / KK, AHEAD = C::RING - 1;
+#pragma unroll
+        for (int i = 1; i < AHEAD; ++i) stage(i, k0 + i);                     // (a slice has RING K steps at least)
+        const _Float16 *fp0 = lds + (wm + fr) * 2 * C::BK, *fq0 = lds + (C::BM + wn + fr) * 2 * C::BK;
+        auto step = [&](const _Float16* p0, const _Float16* q0, auto&& between) {
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            half8 fp[KK][2], fq[KK][2];
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const int at = ((kk * 2 + p * 4 + fk) ^ C::swz(fr)) * 8;
+                    fp[kk][p] = *(const half8*)(p0 + at);
+                    fq[kk][p] = *(const half8*)(q0 + at);
+                }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+                between(kk);
+                low = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[kk][0], fq[kk][1], low, 0, 0, 0);
+                acc[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[kk][0], fq[kk][0], acc[0][0], 0, 0, 0);
+                low = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[kk][1], fq[kk][0], low, 0, 0, 0);
+            }
+        };
+        int kt = k0;
+        for (bool on = true; on;)
+            static_for<C::RING>([&](auto u) {
+                if (!on) return;
+                wait_loads<(AHEAD - 1) * 2 * C::LD>();
+                step(fp0 + u.value * C::STAGE, fq0 + u.value * C::STAGE, [&](int kk) {
+#pragma unroll
+                    for (int e = 0; e < EACH; ++e) load((u.value + AHEAD) % C::RING, kt + AHEAD, (kk * EACH + e) / C::LD, (kk * EACH + e) % C::LD);
+                });
+                on = ++kt + AHEAD < k1;
+            });
+        static_for<AHEAD>([&](auto u) {
+            wait_loads<(AHEAD - 1 - u.value) * 2 * C::LD>();
+            const int buf = (kt + u.value - k0) % C::RING * C::STAGE;
+            step(fp0 + buf, fq0 + buf, [](int) {});
+        });
+    } else
     for (int kt = k0; kt < k1; ++kt) {
         const int buf = (kt - k0) & 1;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (kt + 1 < k1) stage(buf ^ 1, kt + 1);
         const _Float16* base = lds + buf * C::STAGE;
+        auto frag = [&](int side, int row, int kk, int p) {
+            return *(const half8*)(base + (side * C::BM + row) * 2 * C::BK + ((kk * 2 + p * 4 + fk) ^ C::swz(row)) * 8);
+        };
+        if (kt + 1 < k1) stage(buf ^ 1, kt + 1);
 #pragma unroll
         for (int kk = 0; kk < C::BK / 16; ++kk) {
             half8 fp[2][C::MA], fq[2][C::MB];
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
 #pragma unroll
-                for (int a = 0; a < C::MA; ++a) {
-                    const int row = wm + a * 32 + fr;
-                    fp[p][a] = *(const half8*)(base + row * 2 * C::BK + (((kk >> 1) * 8 + p * 4 + (kk & 1) * 2 + fk) ^ C::swz(row)) * 8);
-                }
+                for (int a = 0; a < C::MA; ++a) fp[p][a] = frag(0, wm + a * 32 + fr, kk, p);
 #pragma unroll
-                for (int b = 0; b < C::MB; ++b) {
-                    const int row = wn + b * 32 + fr;
-                    fq[p][b] = *(const half8*)(base + (C::BM + row) * 2 * C::BK + (((kk >> 1) * 8 + p * 4 + (kk & 1) * 2 + fk) ^ C::swz(row)) * 8);
-                }
+                for (int b = 0; b < C::MB; ++b) fq[p][b] = frag(1, wn + b * 32 + fr, kk, p);
             }
 #define FOR_ACC for (int a = 0; a < C::MA; ++a) _Pragma("unroll") for (int b = 0; b < C::MB; ++b)
-            if (ONE) {
-                low = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[0][0], fq[1][0], low, 0, 0, 0);
-                acc[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[0][0], fq[0][0], acc[0][0], 0, 0, 0);
-                low = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[1][0], fq[0][0], low, 0, 0, 0);
-            } else {
 #pragma unroll
-                FOR_ACC acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[0][a], fq[1][b], acc[a][b], 0, 0, 0);
+            FOR_ACC acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[0][a], fq[1][b], acc[a][b], 0, 0, 0);
 #pragma unroll
-                FOR_ACC acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[1][a], fq[0][b], acc[a][b], 0, 0, 0);
+            FOR_ACC acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[1][a], fq[0][b], acc[a][b], 0, 0, 0);
 #pragma unroll
-                FOR_ACC acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[0][a], fq[0][b], acc[a][b], 0, 0, 0);
-            }
+            FOR_ACC acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[0][a], fq[0][b], acc[a][b], 0, 0, 0);
         }
     }
     __syncthreads();
@@ -535,7 +576,8 @@ template <typename C, int KIND> __device__ __forceinline__ void join(const Launc
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[n][h * 4 + e] += v[e];
             }
-    to_lds<C, KIND, false>(s, t, r0, c0, acc, buf, u32x16{});
+    const Quad none[4] = {};
+    to_lds<C, KIND, false>(s, t, r0, c0, acc, buf, none);
     wave_sync();
     leave<C, KIND>(s, t, r0, c0, buf);
 }
@@ -561,7 +603,7 @@ long tiles_of(int kind, long R, long C, int bm) {
 // `two`: while two blocks share the CU) and a block's fixed part; a join reads and writes its slabs once.
 struct Shape { int bm, bk, fit, strips; double one, two, fixed; };
 constexpr Shape SHAPES[3] = {{256, 32, 1, Big::NW * Big::STRIPS, 2.5, 2.5, 30.0}, {128, 32, 2, Mid::NW * Mid::STRIPS, 0.9, 1.6, 10.0},
-                             {64, 64, 2, Small::NW * Small::STRIPS, 0.57, 1.14, 7.0}};
+                             {64, 32, 2, Small::NW * Small::STRIPS, 0.285, 0.57, 7.0}};
 struct Cut { int shape, whole, S; long slab; };               // slab: floats
 Cut cut_of(int kind, long R, long C, long K) {
     Cut best{0, 0, 1, 0};
