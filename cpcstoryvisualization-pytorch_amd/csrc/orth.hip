@@ -21,6 +21,8 @@
 // are padded to whole tiles with zeros, which stay zeros, so that the K loops have no bounds.
 #include "common.h"
 #include "../../include/cpcsv_hip.h"
+#include <algorithm>
+#include <climits>
 
 namespace {
 typedef __attribute__((ext_vector_type(8))) _Float16 half8;
@@ -200,9 +202,11 @@ struct Task {
     int R, C, K;
     float alpha, beta, gamma;
     int shape, t0, tiles, whole, S, r0; // tile shape; first block; tiles, of which `whole` in one piece, the others in S slices of K; first joining block
+    int steps, longer;         // K steps of a slice; slices that have one more
     int rows, cols, tall;                     // OUT, WEIGHT: of the output
 };
 struct Launch {
+    int first[MAXT];           // block of each task (behind the last: none's)
     Task t[MAXT];
     int n, kind, dtype;
     float decay;
@@ -235,25 +239,30 @@ using Mid = Cfg<128, 64, 64, 2>;
 using Small = Cfg<64, 32, 32, 4>;
 static_assert(Big::LDS >= Big::NW * Big::STRIP * 4 && Mid::LDS >= Mid::NW * Mid::STRIP * 4 && Small::LDS >= Small::NW * Small::STRIP * 4, "strips fit");
 
-template <int KIND> __device__ __forceinline__ void tile_of(const Task& t, int tile, int bm, int& ti, int& tj) {
+// of place w in a lower triangle taken row by row (w < 2^20)
+__device__ __forceinline__ unsigned triangle_row(unsigned w) {
+    unsigned r = (unsigned)((__builtin_amdgcn_sqrtf(8.f * (float)w + 1.f) - 1.f) * 0.5f);
+    r -= r * (r + 1) / 2 > w;
+    r += (r + 1) * (r + 2) / 2 <= w;
+    return __builtin_amdgcn_readfirstlane(r);
+}
+template <int KIND> __device__ __forceinline__ void tile_of(const Task& t, unsigned tile, unsigned bm, int& ti, int& tj) {
+    const unsigned tm = (t.R + bm - 1) / bm;
     if (symmetric(KIND)) {
         // lower triangle by blocks of g x g tiles, a row of blocks behind the other (the last one of h tile rows; on the diagonal
         // triangles): a run of tiles shares operand rows in L2. Row by row, every XCD read the whole operand.
-        const int n = (t.R + bm - 1) / bm, g = n >= 24 ? 8 : 4;
-        int I = 0;
-        while ((I + 1) * g < n && (I + 1) * g * ((I + 1) * g + 1) / 2 <= tile) ++I;
-        const int rem = tile - I * g * (I * g + 1) / 2, h = min(g, n - I * g), J = min(rem / (g * h), I), w = rem - J * g * h;
-        if (J < I) { ti = I * g + w / g; tj = J * g + w % g; }
-        else {
-            int r = 0, left = w;
-            while (left > r) { left -= r + 1; ++r; }
-            ti = I * g + r;
-            tj = I * g + left;
-        }
+        const unsigned lg = tm >= 24 ? 3 : 2, g = 1u << lg;
+        const unsigned I = triangle_row(tile) >> lg;           // (the tiles above a row of blocks are as many as row by row)
+        const unsigned rem = tile - I * g * (I * g + 1) / 2, h = min(g, tm - I * g);
+        const unsigned J = min(h == g ? rem >> 2 * lg : rem / (g * h), I), w = rem - J * g * h;
+        const unsigned r = J < I ? w >> lg : triangle_row(w);
+        ti = I * g + r;
+        tj = J * g + w - (J < I ? r * g : r * (r + 1) / 2);
     } else {                                     // bands of 8 tile rows, so that a run of tiles shares operand rows in L2
-        const int tm = (t.R + bm - 1) / bm, tn = (t.C + bm - 1) / bm, g = tile / (8 * tn), gr = min(8, tm - g * 8), w = tile - g * 8 * tn;
-        ti = g * 8 + w % gr;
-        tj = w / gr;
+        const unsigned tn = (t.C + bm - 1) / bm, g = tile / (8 * tn), gr = min(8u, tm - g * 8), w = tile - g * 8 * tn;
+        const unsigned q = gr == 8 ? w >> 3 : w / gr;
+        ti = g * 8 + w - q * gr;
+        tj = q;
     }
 }
 
@@ -370,11 +379,19 @@ template <int KIND> __device__ __forceinline__ bool outside(const Task& t, int r
 // all but the N youngest loads have landed, the wavefront's LDS reads are done
 template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
 
-__device__ __forceinline__ const Task& task_of(const Launch& s) {
-    if (s.n == 1) return s.t[0];
-    // (all first blocks compared at once: a search would be a chain of dependent loads)
-    const int lane = threadIdx.x & 63, first = s.t[min(lane, s.n - 1)].t0;
-    return s.t[__popcll(__ballot(lane < s.n && (int)blockIdx.x >= first)) - 1];
+// The block's task (all first blocks compared at once). task_of: every lane holds one, so that finding it and reading it is one latency
+// of the arguments' memory, half a microsecond; the larger tiles have no registers for that.
+__device__ __forceinline__ int task_at(const Launch& s) {
+    static_assert(MAXT == 32 && sizeof(Task) % 4 == 0 && sizeof(Launch) <= 4096, "a half of the wavefront; a kernel's arguments");
+    return __popc((uint32_t)__ballot((int)blockIdx.x >= s.first[threadIdx.x & 31])) - 1;
+}
+__device__ __forceinline__ Task task_of(const Launch& s) {
+    union { Task t; int w[sizeof(Task) / 4]; } mine, own;
+    mine.t = s.t[threadIdx.x & 31];
+    const int k = task_at(s);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(Task) / 4; ++i) own.w[i] = __builtin_amdgcn_readlane(mine.w[i], k);
+    return own.t;
 }
 
 template <typename C, int KIND>
@@ -384,13 +401,13 @@ __device__ __forceinline__ void product(const Launch& s, const Task& t, unsigned
     // either part, whose operands its L2 then holds, and a share of both
     const bool sliced = (int)blockIdx.x - t.t0 >= t.whole;
     const int from = t.t0 + (sliced ? t.whole : 0), cut = t.tiles - t.whole, n = sliced ? cut * t.S : t.whole, xcd = blockIdx.x & 7;
-    int u = (blockIdx.x - from) >> 3;
-    for (int x = 0; x < xcd; ++x) u += (n + 7 - ((x - from) & 7)) >> 3;
-    const int S = sliced ? t.S : 1, sl = sliced ? u / cut : 0, tile = sliced ? t.whole + u % cut : u;
+    auto more = [&](int v) { return (v >> 3) * (n & 7) + min(v & 7, n & 7); };        // of v XCDs, those that have a block more
+    const int u = ((blockIdx.x - from) >> 3) + xcd * (n >> 3) + more((-from & 7) + xcd) - more(-from & 7);
+    const int S = sliced ? t.S : 1, sl = sliced ? (unsigned)u / (unsigned)cut : 0, tile = sliced ? t.whole + u - sl * cut : u;
     int ti, tj;
     tile_of<KIND>(t, tile, C::BM, ti, tj);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), K = t.K;
-    const int nk = K / C::BK, k0 = (int)((long)nk * sl / S), k1 = (int)((long)nk * (sl + 1) / S);
+    const int k0 = sliced ? sl * t.steps + min(sl, t.longer) : 0, k1 = sliced ? k0 + t.steps + (sl < t.longer) : K / C::BK;
     const _Float16* src[2] = {s.ws + t.p + (long)ti * C::BM * 2 * K, s.ws + t.q + (long)tj * C::BM * 2 * K};
     uint32_t off[2][C::LD];                      // in bytes (K <= 131072 and 256 rows: below 2^28)
 #pragma unroll
@@ -422,7 +439,7 @@ __device__ __forceinline__ void product(const Launch& s, const Task& t, unsigned
 #pragma unroll
             for (int b = 0; b < C::MB; ++b) acc[a][b][e] = 0.f;
     }
-    if (k0 < k1) stage(0, k0);
+    stage(0, k0);
     constexpr bool ONE = C::MA * C::MB == 1;
     Quad early[4] = {};
     if (ONE && KIND == SYMM_E && S == 1) {
@@ -461,7 +478,8 @@ __device__ __forceinline__ void product(const Launch& s, const Task& t, unsigned
             }
         };
         int kt = k0;
-        for (bool on = true; on;)
+        bool on = true;
+        do
             static_for<C::RING>([&](auto u) {
                 if (!on) return;
                 wait_loads<(AHEAD - 1) * 2 * C::LD>();
@@ -471,6 +489,7 @@ __device__ __forceinline__ void product(const Launch& s, const Task& t, unsigned
                 });
                 on = ++kt + AHEAD < k1;
             });
+        while (on);
         static_for<AHEAD>([&](auto u) {
             wait_loads<(AHEAD - 1 - u.value) * 2 * C::LD>();
             const int buf = (kt + u.value - k0) % C::RING * C::STAGE;
@@ -540,16 +559,16 @@ __device__ __forceinline__ void product(const Launch& s, const Task& t, unsigned
 
 // one launch serves the two shapes of 256 threads and 64 KB of LDS
 template <int KIND>
-__global__ __launch_bounds__(Mid::T) void orth_gemm_kernel(Launch s) {
+__global__ __launch_bounds__(Mid::T, 2) void orth_gemm_kernel(Launch s) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const Task& t = task_of(s);
-    if (t.shape == 1) product<Mid, KIND>(s, t, smem);
+    const Task t = task_of(s);
+    if (t.shape == 1) product<Mid, KIND>(s, s.t[task_at(s)], smem);
     else product<Small, KIND>(s, t, smem);
 }
 template <int KIND>
 __global__ __launch_bounds__(Big::T) void orth_gemm_big_kernel(Launch s) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    product<Big, KIND>(s, task_of(s), smem);
+    product<Big, KIND>(s, s.t[task_at(s)], smem);
 }
 
 // the slices of a tile, added in order: one wavefront a strip
@@ -584,8 +603,7 @@ template <typename C, int KIND> __device__ __forceinline__ void join(const Launc
 template <int KIND>
 __global__ __launch_bounds__(64) void orth_join_kernel(Launch s) {
     __shared__ uint32_t buf[Mid::STRIP];
-    const int first = s.t[min((int)threadIdx.x, s.n - 1)].r0;
-    const Task& t = s.t[__popcll(__ballot((int)threadIdx.x < s.n && (int)blockIdx.x >= first)) - 1];
+    const Task t = task_of(s);
     if (t.shape == 0) join<Big, KIND>(s, t, buf);
     else if (t.shape == 1) join<Mid, KIND>(s, t, buf);
     else join<Small, KIND>(s, t, buf);
@@ -676,6 +694,7 @@ template <int KIND> int fire(const Launch& big, const Launch& rest, const Launch
 int run_level(const Launch& all, long slabs, hipStream_t st) {
     Launch big = all, rest = all, join = all;
     big.n = rest.n = join.n = 0;
+    for (Launch* l : {&big, &rest, &join}) std::fill(l->first, l->first + MAXT, INT_MAX);
     long at = 0, units[2] = {0, 0}, joins = 0;
     for (int i = 0; i < all.n; ++i) {
         Task t = all.t[i];
@@ -683,15 +702,16 @@ int run_level(const Launch& all, long slabs, hipStream_t st) {
         t.shape = cut.shape;
         t.tiles = (int)tiles_of(all.kind, t.R, t.C, SHAPES[cut.shape].bm);
         t.whole = cut.whole; t.S = cut.S; t.slab = at;
+        t.steps = t.K / SHAPES[cut.shape].bk / t.S; t.longer = t.K / SHAPES[cut.shape].bk % t.S;
         at += cut.slab;
         long& u = units[cut.shape != 0];
         t.t0 = (int)u; t.r0 = (int)joins;
         u += t.whole + (long)(t.tiles - t.whole) * t.S;
         if (t.S > 1) joins += (long)(t.tiles - t.whole) * SHAPES[cut.shape].strips;
         if (u > (1L << 30) || joins > (1L << 30)) return -1002;
-        Launch& to = cut.shape ? rest : big;
-        to.t[to.n++] = t;
-        if (t.S > 1) join.t[join.n++] = t;
+        auto put = [&](Launch& l, int first) { l.first[l.n] = first; l.t[l.n++] = t; };
+        put(cut.shape ? rest : big, t.t0);
+        if (t.S > 1) put(join, t.r0);
     }
     if (at > slabs) return -1004;
     switch (all.kind) {
