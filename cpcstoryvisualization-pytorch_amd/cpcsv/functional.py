@@ -1372,6 +1372,12 @@ def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _once(backward):
+    """once_differentiable, whose bookkeeping (5 us a call) runs only where a graph of the gradients is asked for."""
+    recorded = once_differentiable(backward)
+    return lambda ctx, *grads: recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+
 def _scan_args(p, h0, lengths, out_gate, rank):
     """Checks of gated_scan / gated_scan_step -> H."""
     k, shape = 3 if out_gate else 2, p.shape
@@ -1412,8 +1418,9 @@ def _scan_forward(p, h0, lengths, out_gate, keep):
     if b == 0 or t == 0:
         last.copy_(h0) if h0 is not None else last.zero_()
     else:
-        if keep and K.scan_states(t):
-            hin = _empty((b, K.scan_states(t), h), torch.float32, dev)
+        states = K.scan_states(t) if keep else 0
+        if states:
+            hin = _empty((b, states, h), torch.float32, dev)
         ws = K.scan_fwd(p, h0, lengths, y, last, hin, b, t, h, out_gate)
         _runtime.keep_forced(p, h0, lengths, hin, ws)
     return y, last, p, h0, lengths, hin
@@ -1431,7 +1438,7 @@ class GatedScanFn(Function):
         return y, last
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy, dlast):
         p, h0, lengths, hin = ctx.saved_tensors
         b, t, h = p.shape[0], p.shape[1], p.shape[2] // (3 if ctx.out_gate else 2)
@@ -1520,7 +1527,7 @@ class NormResidualFn(Function):
         return outs
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, *grads):
         x, u, w_post, gate, scale, w_next, ru, rx = ctx.saved_tensors
         rows, d, udt, mode, t = ctx.geom

@@ -191,3 +191,17 @@ def test_modules_refuse():
             rec(x)
     with pytest.raises(ValueError, match="GatedRecurrence"):
         rec.step(torch.zeros(2, 3, 8).cuda(), torch.zeros(2, 4).cuda())
+
+
+def test_gradients_of_gradients_are_refused():
+    """create_graph=True gives first derivatives; a second one through the operators raises."""
+    from cpcsv import functional as F
+    p = torch.randn(2, 40, 12, device="cuda", requires_grad=True)
+    x = torch.randn(2, 40, 4, device="cuda", requires_grad=True)
+    w = torch.ones(4, device="cuda")
+    for f, leaf in ((lambda: F.gated_scan(p)[0], p), (lambda: F.norm_residual(x, x, w), x), (lambda: F.rms_norm(x, w), x)):
+        want, = torch.autograd.grad(f().square().sum(), leaf)
+        got, = torch.autograd.grad(f().square().sum(), leaf, create_graph=True)
+        assert torch.equal(got, want)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            got.sum().backward()
