@@ -52,10 +52,11 @@ struct Jobs {
     _Float16* ws;
 };
 
-template <int Job::*FIRST> __device__ __forceinline__ int job_of(const Jobs& s, int block) {
-    int k = 0;
-    while (k + 1 < s.n && block >= s.j[k + 1].*FIRST) ++k;
-    return k;
+// all first blocks compared at once (a search is a chain of loads that wait half a microsecond each)
+template <int Job::*FIRST> __device__ __forceinline__ int job_of(const Jobs& s) {
+    static_assert(MAXJ == 16, "a quarter of the wavefront");
+    const int l = threadIdx.x & 15, first = s.j[l].*FIRST;                   // (behind the last job: 0)
+    return __popc((uint32_t)__ballot((int)blockIdx.x >= first && (first || !l)) & 0xffff) - 1;
 }
 __device__ __forceinline__ float ld_g(const void* p, int dtype, long i) {
     return dtype == CPCSV_F32 ? ((const float*)p)[i] : bf16_to_f32(((const bf16_t*)p)[i]);
@@ -85,7 +86,7 @@ __host__ __device__ inline int norm_blocks(int rows, int cols) {
 
 // ---- momentum and |U|^2 (double: squares of any fp32 value) ----------------------------------------------------------
 __global__ __launch_bounds__(256) void orth_norm_kernel(Jobs s) {
-    const int k = job_of<&Job::t_norm>(s, blockIdx.x);
+    const int k = job_of<&Job::t_norm>(s);
     const Job& j = s.j[k];
     const int blk = blockIdx.x - j.t_norm, nb = norm_blocks(j.rows, j.cols);
     const long n = (long)j.rows * j.cols;
@@ -146,8 +147,20 @@ __global__ __launch_bounds__(256) void orth_norm_kernel(Jobs s) {
 __global__ __launch_bounds__(256) void orth_split_kernel(Jobs s) {
     __shared__ uint32_t t[64][65];
     __shared__ double sh[256];
-    const int k = job_of<&Job::t_split>(s, blockIdx.x);
+    const int k = job_of<&Job::t_split>(s);
     const Job& j = s.j[k];
+    const int PR = j.tall ? j.N : j.M, PC = j.tall ? j.M : j.N, tile = blockIdx.x - j.t_split;
+    const int r0 = tile / (PC / 64) * 64, c0 = tile % (PC / 64) * 64;
+    const int cl = threadIdx.x & 63, rl = threadIdx.x >> 6, c = c0 + cl;
+    float u[16], m[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int r = r0 + i * 4 + rl;
+        const bool in = r < j.rows && c < j.cols;
+        const long at = in ? (long)r * j.cols + c : 0;
+        u[i] = in ? ld_g(j.g, s.dtype, at) : 0.f;
+        m[i] = in && j.m ? j.m[at] : 0.f;
+    }
     double sum = 0.0;
     for (int i = threadIdx.x; i < norm_blocks(j.rows, j.cols); i += 256) sum += s.part[k * NORMB + i];
     sh[threadIdx.x] = sum;
@@ -157,20 +170,11 @@ __global__ __launch_bounds__(256) void orth_split_kernel(Jobs s) {
         __syncthreads();
     }
     const float inv = (float)((double)SX / (sqrt(sh[0]) + (double)s.eps));
-    const int PR = j.tall ? j.N : j.M, PC = j.tall ? j.M : j.N, tile = blockIdx.x - j.t_split;
-    const int r0 = tile / (PC / 64) * 64, c0 = tile % (PC / 64) * 64;
-    const int cl = threadIdx.x & 63, rl = threadIdx.x >> 6;
-#pragma unroll 4
+#pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const int r = r0 + i * 4 + rl, c = c0 + cl;
-        float u = 0.f;
-        if (r < j.rows && c < j.cols) {
-            const long at = (long)r * j.cols + c;
-            u = ld_g(j.g, s.dtype, at);
-            if (j.m) u = s.nesterov ? __fmaf_rn(s.mu, j.m[at], u) : j.m[at];
-            u *= inv;
-        }
-        t[i * 4 + rl][cl] = split_of(u);
+        const float v = !j.m ? u[i] : s.nesterov ? __fmaf_rn(s.mu, m[i], u[i]) : m[i];
+        const bool in = r0 + i * 4 + rl < j.rows && c < j.cols;
+        t[i * 4 + rl][cl] = split_of(in ? v * inv : 0.f);
     }
     __syncthreads();
     _Float16 *own = s.ws + (j.tall ? j.xt : j.x), *turned = s.ws + (j.tall ? j.x : j.xt);
