@@ -8,8 +8,10 @@
 // it, and exactly the forward's fp32 value rather than its rounded copy), the row statistics are two floats a row.
 // A row is owned by `tpr` threads (64: one wavefront, no barrier; up to 1024 for wide rows) that keep 8 values each in registers
 // between the two reductions, with their share of the weights beside them: blocks walk many rows, so the weights are read once a
-// block, and the next row is loaded before this one's reductions. The weight gradients' column sums accumulate in registers over a
-// block's rows and are joined by a second launch in a fixed order.
+// block, and the next row is loaded before this one's reductions. 32768 rows of 2048 in bf16 with a gate a token: forward 135 us,
+// 5.0 TB/s; backward 224 us, 4.8 TB/s (a large copy: 4.9 to 5.4). 8192 rows of 8192, an fp32 stream: 182 and 289 us, 4.4 and 4.2 TB/s.
+// The weight gradients' column sums accumulate in registers over a block's rows and are joined by a second launch (8 us) in a fixed
+// order.
 #include "common.h"
 #include "../../include/cpcsv_hip.h"
 
