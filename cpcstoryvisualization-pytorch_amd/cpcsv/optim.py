@@ -333,7 +333,10 @@ class FusedMuon(torch.optim.Optimizer):
 
     def add_param_group(self, group):
         super().add_param_group(group)
-        for p in self.param_groups[-1]["params"]:
+        params = self.param_groups[-1]["params"]
+        if len(set(params)) < len(params):
+            raise ValueError("FusedMuon: a parameter stands twice in a group (its two updates would run at once)")
+        for p in params:
             if p.dim() < 2:
                 raise ValueError("FusedMuon takes matrices (two or more dimensions), got shape %s: leave vectors to FusedAdam" % (tuple(p.shape),))
             _side_ok(self._matrix(p), "FusedMuon")

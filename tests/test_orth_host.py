@@ -41,6 +41,8 @@ def test_muon_refuses():
         FusedMuon([w, torch.nn.Parameter(torch.zeros(6))])
     with pytest.raises(ValueError, match="sides of"):
         FusedMuon([torch.nn.Parameter(torch.zeros(0, 6))])
+    with pytest.warns(UserWarning, match="duplicate"), pytest.raises(ValueError, match="twice"):
+        FusedMuon([w, w])
     w.grad = torch.zeros_like(w)
     with pytest.raises(RuntimeError, match="contiguous fp32 GPU"):
         FusedMuon([w]).step()
