@@ -449,12 +449,6 @@ __device__ __forceinline__ void product(const Launch& s, const Task& t, unsigned
     stage(0, k0);
     constexpr bool ONE = C::MA * C::MB == 1;
     Quad early[4] = {};
-    if (ONE && KIND == SYMM_E && S == 1) {
-        const int r0 = ti * C::BM + wm, c0 = tj * C::BM + wn;
-        if (r0 < t.R && c0 < t.C)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) early[g] = quad_of(s, t, r0 + g * 8 + fk * 4, c0 + fr);
-    }
     if constexpr (ONE) {
         // One wavefront a SIMD: what bounds a step is what it has to issue. Unrolled over the ring, so that LDS addresses are constants;
         // all fragments first, the loads between the MFMAs; the RING - 1 stages in flight are behind a barrier of its own (one with
@@ -462,6 +456,12 @@ __device__ __forceinline__ void product(const Launch& s, const Task& t, unsigned
         constexpr int KK = C::BK / 16, EACH = 2 * C::LD / KK, AHEAD = C::RING - 1;
 #pragma unroll
         for (int i = 1; i < AHEAD; ++i) stage(i, k0 + i);                     // (a slice has RING K steps at least)
+        if (KIND == SYMM_E && S == 1) {              // behind the stages: scattered over 32 rows, they come late
+            const int r0 = ti * C::BM + wm, c0 = tj * C::BM + wn;
+            if (r0 < t.R && c0 < t.C)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) early[g] = quad_of(s, t, r0 + g * 8 + fk * 4, c0 + fr);
+        }
         const _Float16 *fp0 = lds + (wm + fr) * 2 * C::BK, *fq0 = lds + (C::BM + wn + fr) * 2 * C::BK;
         auto step = [&](const _Float16* p0, const _Float16* q0, auto&& between) {
             __builtin_amdgcn_s_barrier();
