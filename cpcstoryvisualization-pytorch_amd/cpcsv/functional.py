@@ -31,7 +31,11 @@ def _empty(shape, dtype, dev, zero=False):
 def _empty_like(t):
     """torch.empty_like; CPCSV_POISON=1 fills with NaN so a read of a never-written element surfaces in the tests."""
     r = torch.empty_like(t)
-    return r.fill_(float("nan")) if _POISON and r.is_floating_point() else r
+    return r.fill_(float("nan")) if r.is_floating_point() else r
+
+
+if not _POISON:
+    _empty_like = torch.empty_like
 
 
 # ------------------------------------------------------------------------------------------------
@@ -1505,15 +1509,14 @@ def _norm_forward(x, u, w_post, gate, scale, w_next, out_dtype, eps, keep):
         mode, t = (1, 1) if per == rows else (2, rows // per)
     xo = _empty_like(x) if u is not None else None
     z = (_empty_like(x) if out_dtype == x.dtype else _empty(x.shape, out_dtype, dev)) if w_next is not None else None
-    ru = rx = None
+    stats = None
     if rows:
         if keep:
-            ru = _empty((rows,), torch.float32, dev) if u is not None else None
-            rx = _empty((rows,), torch.float32, dev) if w_next is not None else None
-        K.norm_residual_fwd(x, u, gate, scale, w_post, w_next, xo, z, ru, rx, rows, d, udt, mode, t, eps)
-        _runtime.keep_forced(x, u, gate, w_post, scale, w_next, ru, rx)
+            stats = _empty(((u is not None) + (w_next is not None), rows), torch.float32, dev)
+        K.norm_residual_fwd(x, u, gate, scale, w_post, w_next, xo, z, stats, rows, d, udt, mode, t, eps)
+        _runtime.keep_forced(x, u, gate, w_post, scale, w_next, stats)
     outs = (xo, z) if xo is not None and z is not None else (xo if xo is not None else z)
-    return outs, (x, u, w_post, gate, scale, w_next, ru, rx), (rows, d, udt, mode, t)
+    return outs, (x, u, w_post, gate, scale, w_next, stats), (rows, d, udt, mode, t)
 
 
 class NormResidualFn(Function):
@@ -1529,7 +1532,7 @@ class NormResidualFn(Function):
     @staticmethod
     @_once
     def backward(ctx, *grads):
-        x, u, w_post, gate, scale, w_next, ru, rx = ctx.saved_tensors
+        x, u, w_post, gate, scale, w_next, stats = ctx.saved_tensors
         rows, d, udt, mode, t = ctx.geom
         if len(grads) == 2:
             dxo, dz = grads
@@ -1558,7 +1561,7 @@ class NormResidualFn(Function):
         part = None
         if dwp is not None or dsc is not None or dwn is not None or (mode == 2 and dgate is not None):
             part = _empty((K.norm_residual_part(rows, d, mode, t),), torch.float32, x.device)
-        K.norm_residual_bwd(x, u, gate, scale, w_post, w_next, ru, rx, dxo, dz, dx, du, dgate, dsc, dwp, dwn, part, rows, d, udt, mode, t)
+        K.norm_residual_bwd(x, u, gate, scale, w_post, w_next, stats, dxo, dz, dx, du, dgate, dsc, dwp, dwn, part, rows, d, udt, mode, t)
         _runtime.keep_forced(dxo, dz, part)
         return dx, du, dwp, dgate, dsc, dwn, None, None
 

@@ -613,11 +613,14 @@ def _scan_ws(B, T, H, backward, dev):
     return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
 
 
+# (these four are what a small training call waits for: pointers are taken in place, ptr() is a call each)
 def scan_fwd(p, h0, lengths, y, h_last, hin, B, T, H, out_gate):
     """Returns the call's scratch (None for short sequences)."""
     ws = _scan_ws(B, T, H, 0, p.device)
-    _call("cpcsv_scan_fwd", ptr(p), dcode(p), p.stride(0), p.stride(1), ptr(h0), ptr(lengths), ptr(y), ptr(h_last), ptr(hin), ptr(ws),
-          B, T, H, int(out_gate), stream())
+    sb, st, _ = p.stride()
+    _call("cpcsv_scan_fwd", p.data_ptr(), dcode(p), sb, st, h0.data_ptr() if h0 is not None else None,
+          lengths.data_ptr() if lengths is not None else None, y.data_ptr(), h_last.data_ptr(), hin.data_ptr() if hin is not None else None,
+          ws.data_ptr() if ws is not None else None, B, T, H, out_gate, stream())
     return ws
 
 
@@ -630,24 +633,44 @@ def scan_step(p, h, y, B, H, out_gate):
 def scan_bwd(p, h0, lengths, hin, dy, dh_last, dp, dh0, B, T, H, out_gate):
     """Returns the call's scratch (None for short sequences)."""
     ws = _scan_ws(B, T, H, 1, p.device)
-    _call("cpcsv_scan_bwd", ptr(p), dcode(p), p.stride(0), p.stride(1), ptr(h0), ptr(lengths), ptr(hin), ptr(dy), ptr(dh_last), ptr(dp),
-          ptr(dh0), ptr(ws), B, T, H, int(out_gate), stream())
+    sb, st, _ = p.stride()
+    _call("cpcsv_scan_bwd", p.data_ptr(), dcode(p), sb, st, h0.data_ptr() if h0 is not None else None,
+          lengths.data_ptr() if lengths is not None else None, hin.data_ptr() if hin is not None else None, dy.data_ptr(),
+          dh_last.data_ptr() if dh_last is not None else None, dp.data_ptr(), dh0.data_ptr() if dh0 is not None else None,
+          ws.data_ptr() if ws is not None else None, B, T, H, out_gate, stream())
     return ws
 
 
-def norm_residual_fwd(x, u, gate, scale, w_post, w_next, xo, z, ru, rx, rows, D, udt, gate_mode, T, eps):
-    _call("cpcsv_norm_residual_fwd", ptr(x), ptr(u), ptr(gate), ptr(scale), ptr(w_post), ptr(w_next), ptr(xo), ptr(z), ptr(ru), ptr(rx),
-          rows, D, dcode(x), udt, gate_mode, T, float(eps), stream())
+def _stat_ptrs(stats, u, w_next, rows):
+    """stats fp32 [1 or 2][rows]: u's 1/rms, then x's; of those that are there."""
+    if stats is None:
+        return None, None
+    at = stats.data_ptr()
+    return (at if u is not None else None), (None if w_next is None else at + 4 * rows if u is not None else at)
+
+
+def norm_residual_fwd(x, u, gate, scale, w_post, w_next, xo, z, stats, rows, D, udt, gate_mode, T, eps):
+    ru, rx = _stat_ptrs(stats, u, w_next, rows)
+    _call("cpcsv_norm_residual_fwd", x.data_ptr(), u.data_ptr() if u is not None else None, gate.data_ptr() if gate is not None else None,
+          scale.data_ptr() if scale is not None else None, w_post.data_ptr() if w_post is not None else None,
+          w_next.data_ptr() if w_next is not None else None, xo.data_ptr() if xo is not None else None, z.data_ptr() if z is not None else None,
+          ru, rx, rows, D, dcode(x), udt, gate_mode, T, eps, stream())
 
 
 def norm_residual_part(rows, D, gate_mode, T):
     return L.load().cpcsv_norm_residual_part(rows, D, gate_mode, T)
 
 
-def norm_residual_bwd(x, u, gate, scale, w_post, w_next, ru, rx, dxo, dz, dx, du, dgate, dscale, dw_post, dw_next, part, rows, D, udt,
+def norm_residual_bwd(x, u, gate, scale, w_post, w_next, stats, dxo, dz, dx, du, dgate, dscale, dw_post, dw_next, part, rows, D, udt,
                       gate_mode, T):
-    _call("cpcsv_norm_residual_bwd", ptr(x), ptr(u), ptr(gate), ptr(scale), ptr(w_post), ptr(w_next), ptr(ru), ptr(rx), ptr(dxo), ptr(dz),
-          ptr(dx), ptr(du), ptr(dgate), ptr(dscale), ptr(dw_post), ptr(dw_next), ptr(part), rows, D, dcode(x), udt, gate_mode, T, stream())
+    ru, rx = _stat_ptrs(stats, u, w_next, rows)
+    _call("cpcsv_norm_residual_bwd", x.data_ptr(), u.data_ptr() if u is not None else None, gate.data_ptr() if gate is not None else None,
+          scale.data_ptr() if scale is not None else None, w_post.data_ptr() if w_post is not None else None,
+          w_next.data_ptr() if w_next is not None else None, ru, rx, dxo.data_ptr() if dxo is not None else None,
+          dz.data_ptr() if dz is not None else None, dx.data_ptr(), du.data_ptr() if du is not None else None,
+          dgate.data_ptr() if dgate is not None else None, dscale.data_ptr() if dscale is not None else None,
+          dw_post.data_ptr() if dw_post is not None else None, dw_next.data_ptr() if dw_next is not None else None,
+          part.data_ptr() if part is not None else None, rows, D, dcode(x), udt, gate_mode, T, stream())
 
 
 def _orth_lists(*lists):

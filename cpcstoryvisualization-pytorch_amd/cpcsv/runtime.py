@@ -377,12 +377,16 @@ def require_gpu(t):
 
 def require_here(*tensors):
     """Every tensor (None is skipped) is on the current GPU: kernels go to the current device's stream."""
+    here = None
     for t in tensors:
-        if t is not None:
+        if t is None:
+            continue
+        at = t.get_device()                        # (-1 on the CPU)
+        if here is None and at >= 0:
+            here = _current_device()
+        if at != here:
             require_gpu(t)
-            if t.get_device() != _current_device():
-                raise RuntimeError("tensor on %s while the current device is cuda:%d: call inside `with torch.cuda.device(...)`"
-                                   % (t.device, _current_device()))
+            raise RuntimeError("tensor on %s while the current device is cuda:%d: call inside `with torch.cuda.device(...)`" % (t.device, here))
 
 
 def keep_forced(*tensors):
