@@ -452,7 +452,8 @@ __device__ __forceinline__ void product(const Launch& s, const Task& t, unsigned
     if constexpr (ONE) {
         // One wavefront a SIMD: what bounds a step is what it has to issue. Unrolled over the ring, so that LDS addresses are constants;
         // all fragments first, the loads between the MFMAs; the RING - 1 stages in flight are behind a barrier of its own (one with
-        // the compiler's fence would wait for them). 475 cycles a step, 384 of them LDS traffic; 725 with two stages and a loop.
+        // the compiler's fence would wait for them). 475 cycles a step, 384 of them LDS traffic, 550 where half the CUs are at work (16 KB
+        // a step arrive at 30 bytes a cycle and CU); 725 with two stages and a loop.
         constexpr int KK = C::BK / 16, EACH = 2 * C::LD / KK, AHEAD = C::RING - 1;
 #pragma unroll
         for (int i = 1; i < AHEAD; ++i) stage(i, k0 + i);                     // (a slice has RING K steps at least)
