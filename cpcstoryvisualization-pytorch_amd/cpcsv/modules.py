@@ -212,6 +212,9 @@ TERM_LOG = None        # list while a sub-graph is captured: spectral-norm terms
 USE_LOG = None         # list while a sub-graph is captured: EVERY operand set the captured kernels read (graphs.py)
 
 
+STEPPED, REPLAYED = 1, 2       # weight._cpcsv_moves: its optimiser (cpcsv.optim.FusedMuon) steps it | from inside a captured graph
+
+
 class KernelLayer:
     """Static description + operand caches of one conv/linear(+BN)(+act) node."""
 
@@ -244,8 +247,13 @@ class KernelLayer:
 
     @staticmethod
     def pack_key(weight, dt):
-        # _version catches torch-side in-place updates; _cpcsv_epoch is bumped by FusedAdam, whose kernel
-        # writes through raw pointers and is invisible to torch's version counter
+        # _version catches torch-side in-place updates; _cpcsv_epoch is bumped by the fused optimisers, whose kernels
+        # write through raw pointers and are invisible to torch's version counter. Neither moves when a replayed graph writes
+        # the weight, and a graph that was captured on copies found fresh would never rebuild them: in both cases the copies
+        # count as stale (a key that equals none)
+        moves = getattr(weight, "_cpcsv_moves", 0)
+        if moves and (moves == REPLAYED or torch.cuda.is_current_stream_capturing()):
+            return (object(),)
         return (weight.data_ptr(), weight._version, getattr(weight, "_cpcsv_epoch", 0), dt)
 
     def packs(self, weight, dt, which="both"):

@@ -311,13 +311,21 @@ def orthogonalize(g, steps=5, eps=1e-7):
     return out
 
 
+def _note_moves(params, captured):
+    """What cpcsv.modules.KernelLayer.pack_key has to know of a weight that graph replays may move."""
+    from .modules import REPLAYED, STEPPED
+    for p in params:
+        p._cpcsv_moves = max(getattr(p, "_cpcsv_moves", 0), REPLAYED if captured else STEPPED)
+
+
 class FusedMuon(torch.optim.Optimizer):
     """Momentum, orthogonalised: for weights that act as matrices (dense, convolution - seen as [out, inputs x taps] -, recurrent).
         m <- momentum m + g;  U = g + momentum m (nesterov) or m;  X = orthogonalize(U);
         w <- w (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) X
     Up to 16 matrices share each of the 3 steps + 2 launches (csrc/orth.hip); biases, norms and other vectors belong to FusedAdam. Like
-    there the learning rate lives on the device (graph replays follow sync_lr()), operand caches of the weights are invalidated, and
-    parameters, gradients and momentum are contiguous fp32 GPU tensors."""
+    there the learning rate lives on the device (graph replays follow sync_lr()), and parameters, gradients and momentum are contiguous
+    fp32 GPU tensors. Operand copies that layers keep of these weights are made anew after a step; once a step has been captured,
+    and inside every graph that a user captures, at each use, since nothing tells the host when a replay has moved the weights."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, eps=1e-7):
         if not lr >= 0 or not 0 <= momentum < 1 or not weight_decay >= 0 or not eps >= 0:
@@ -330,6 +338,8 @@ class FusedMuon(torch.optim.Optimizer):
     def __setstate__(self, state):               # (copies and unpickled optimisers; load_state_dict comes here too and keeps the scalars)
         super().__setstate__(state)
         self.__dict__.setdefault("_hypers", {})
+        for group in self.param_groups:
+            _note_moves(group["params"], False)
 
     def add_param_group(self, group):
         super().add_param_group(group)
@@ -340,6 +350,7 @@ class FusedMuon(torch.optim.Optimizer):
             if p.dim() < 2:
                 raise ValueError("FusedMuon takes matrices (two or more dimensions), got shape %s: leave vectors to FusedAdam" % (tuple(p.shape),))
             _side_ok(self._matrix(p), "FusedMuon")
+        _note_moves(params, False)
 
     @staticmethod
     def _matrix(p):
@@ -395,4 +406,5 @@ class FusedMuon(torch.optim.Optimizer):
                 R.keep_forced(ws)
             for p in plist:      # invalidate packed-operand caches (cpcsv.modules.KernelLayer.packs)
                 p._cpcsv_epoch = getattr(p, "_cpcsv_epoch", 0) + 1
+            _note_moves(plist, torch.cuda.is_current_stream_capturing())
         return loss

@@ -1,0 +1,124 @@
+"""Calls that the documentation of the gated recurrence, the block norms and the orthogonalised updates allows beside the ordinary ones
+(csrc/scan.hip, csrc/blocknorm.hip, csrc/orth.hip): each gives the definition's values or is refused, none goes wrong without a word."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def dense_error(y, x, w, b, cast):
+    """|y - (x w^T + b)| over its bound: operands rounded once to `cast` (half a step each), sums of K products in fp32, y stored in fp32."""
+    x, w, b = x.detach().double().cpu(), w.detach().double().cpu(), b.detach().double().cpu()
+    u = 0.0 if cast == torch.float32 else torch.finfo(cast).eps
+    lim = (x.abs() @ w.abs().T) * (u * (1 + u) + (x.shape[1] + 2) * 2.0 ** -24) + b.abs() * 2.0 ** -23
+    return ((y.detach().double().cpu() - (x @ w.T + b)).abs() / lim).max().item()
+
+
+def muon_layer(cin, cout, opt_cls="FusedMuon"):
+    """-> layer, its weight, a step with a constant gradient that moves every entry visibly"""
+    from cpcsv import modules as M, optim
+    torch.manual_seed(3)
+    layer = M.FusedSequential(M.Linear(cin, cout), out_mode="f32").cuda()
+    w = layer[0].weight
+    w.grad = torch.randn_like(w)
+    opt = getattr(optim, opt_cls)([w], lr=0.5)
+    return layer, w, layer[0].bias, opt
+
+
+@pytest.fixture
+def bf16():
+    from cpcsv import runtime
+    keep = runtime.compute_dtype_name()
+    runtime.set_compute_dtype("bf16")
+    yield
+    runtime.set_compute_dtype(keep)
+
+
+@pytest.mark.parametrize("cin,cout,cast", [(40, 24, torch.float32), (2048, 1032, torch.bfloat16)])
+def test_eager_layers_follow_replayed_steps(cin, cout, cast, bf16):
+    """Only the optimiser's step is captured: every eager forward and backward behind a replay multiplies with the weights of that replay
+    (small layers in fp32, larger ones through copies in the compute type)."""
+    layer, w, b, opt = muon_layer(cin, cout)
+    opt.step()
+    x = torch.randn(70, cin, device="cuda", requires_grad=True)
+    dy = torch.randn(70, cout, device="cuda")
+
+    def check():
+        y = layer(x)
+        assert dense_error(y, x, w, b, cast) <= 1
+        gx, = torch.autograd.grad(y, x, dy)
+        dyc = dy.to(cast).float()
+        assert dense_error(gx, dyc, w.T, torch.zeros(cin, device="cuda"), cast) <= 1 if cast == torch.float32 else \
+            (gx - dyc @ w.to(cast).float()).abs().max() <= 2.0 ** -7 * (dyc.abs() @ w.abs()).max()
+    check()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    check()
+    for _ in range(3):
+        before = w.detach().clone()
+        graph.replay()
+        check()
+        assert (w - before).norm() > 0.01 * before.norm()
+    opt.step()
+    check()
+
+
+@pytest.mark.parametrize("first", [True, False])
+def test_captured_layers_follow_later_steps(first, bf16):
+    """A captured forward (here without a step in it) reads the weights of its replay, whether the copies it multiplies with were there
+    before the capture or not."""
+    layer, w, b, opt = muon_layer(40, 24)
+    x = torch.randn(70, 40, device="cuda")
+    with torch.no_grad():
+        layer(x)
+        if first:
+            opt.step()
+        layer(x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = layer(x)
+        for _ in range(3):
+            opt.step()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert dense_error(y, x, w, b, torch.float32) <= 1
+            assert dense_error(layer(x), x, w, b, torch.float32) <= 1
+
+
+def test_a_captured_training_step_and_eager_evaluations(bf16):
+    """Forward, backward and step in one graph, captured behind an eager evaluation, an evaluation behind each replay: the weights and
+    outputs of the same steps run eagerly."""
+    runs = []
+    for captured in (False, True):
+        layer, w, b, opt = muon_layer(40, 24)
+        gen = torch.Generator("cuda").manual_seed(9)
+        x, dy = torch.randn(70, 40, generator=gen, device="cuda"), torch.randn(70, 24, generator=gen, device="cuda")
+        w.grad.zero_()
+
+        def step():
+            g, = torch.autograd.grad(layer(x), w, dy)
+            w.grad.copy_(g)
+            opt.step()
+
+        def evaluate():
+            with torch.no_grad():
+                return layer(x).clone()
+        for _ in range(2):
+            step()
+        outs = [evaluate()]
+        if captured:
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                step()
+        for _ in range(3):
+            graph.replay() if captured else step()
+            torch.cuda.synchronize()
+            outs.append(evaluate())
+            assert dense_error(outs[-1], x, w, b, torch.float32) <= 1
+        runs.append(outs + [w.detach().clone()])
+    for a, c in zip(*runs):
+        assert torch.equal(a, c)
