@@ -212,7 +212,7 @@ TERM_LOG = None        # list while a sub-graph is captured: spectral-norm terms
 USE_LOG = None         # list while a sub-graph is captured: EVERY operand set the captured kernels read (graphs.py)
 
 
-STEPPED, REPLAYED = 1, 2       # weight._cpcsv_moves: its optimiser (cpcsv.optim.FusedMuon) steps it | from inside a captured graph
+STEPPED, REPLAYED = 1, 2       # weight._cpcsv_moves: cpcsv.optim.FusedMuon steps it | a captured step of either optimiser does
 
 
 class KernelLayer:

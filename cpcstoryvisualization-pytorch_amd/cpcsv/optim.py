@@ -15,6 +15,13 @@ from . import runtime as R
 from .runtime import dcode
 
 
+def _note_moves(params, captured):
+    """What cpcsv.modules.KernelLayer.pack_key has to know of a weight that graph replays may move."""
+    from .modules import REPLAYED, STEPPED
+    for p in params:
+        p._cpcsv_moves = max(getattr(p, "_cpcsv_moves", 0), REPLAYED if captured else STEPPED)
+
+
 class FusedAdam(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps))
@@ -275,6 +282,8 @@ class FusedAdam(torch.optim.Optimizer):
             K.adam_step(ptrs, sizes, nt, nchunks, ctens, coff, hyper, b1, b2, group["eps"])
             for p in plist:      # invalidate packed-operand caches (cpcsv.modules.KernelLayer.packs)
                 p._cpcsv_epoch = getattr(p, "_cpcsv_epoch", 0) + 1
+            if torch.cuda.is_current_stream_capturing():
+                _note_moves(plist, True)
             if gi == 0 and self._layers:
                 self._step_layers(group, hyper, pending, gscale, wire_of)        # reads the step count the launch above just advanced
         return loss
@@ -309,13 +318,6 @@ def orthogonalize(g, steps=5, eps=1e-7):
         ws = K.orthogonalize(part, outs[i:i + L.ORTH_JOBS], [tuple(q.shape) for q in part], int(steps), eps)
         R.keep_forced(src, out, ws)
     return out
-
-
-def _note_moves(params, captured):
-    """What cpcsv.modules.KernelLayer.pack_key has to know of a weight that graph replays may move."""
-    from .modules import REPLAYED, STEPPED
-    for p in params:
-        p._cpcsv_moves = max(getattr(p, "_cpcsv_moves", 0), REPLAYED if captured else STEPPED)
 
 
 class FusedMuon(torch.optim.Optimizer):

@@ -122,3 +122,20 @@ def test_a_captured_training_step_and_eager_evaluations(bf16):
         runs.append(outs + [w.detach().clone()])
     for a, c in zip(*runs):
         assert torch.equal(a, c)
+
+
+def test_eager_layers_follow_replayed_adam_steps(bf16):
+    """The same of FusedAdam's captured step."""
+    layer, w, b, opt = muon_layer(40, 24, "FusedAdam")
+    x = torch.randn(70, 40, device="cuda")
+    opt.step()
+    layer(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(3):
+        before = w.detach().clone()
+        graph.replay()
+        assert dense_error(layer(x), x, w, b, torch.float32) <= 1
+        assert not torch.equal(w, before)
