@@ -8,7 +8,7 @@ cpcsv/modules.py and model.py.
 import os
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad as _fw
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -1373,7 +1373,9 @@ class GruSeqFn(Function):
 # gated linear recurrence
 # ------------------------------------------------------------------------------------------------
 def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether a call has to go through its autograd function: it records a gradient, or a dual level is open (a tensor with a tangent does
+    not require grad; the function refuses it, a result without a tangent would count as a zero derivative)."""
+    return _fw._current_level >= 0 or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
 
 
 def _once(backward):
@@ -1478,8 +1480,9 @@ def gated_scan(p, h0=None, lengths=None, out_gate=True):
 
 def gated_scan_step(p, h, out_gate=True):
     """One token of gated_scan for every row: p [B, 3H] (2H without the output gate), h fp32 [B, H] contiguous, UPDATED IN PLACE.
-    -> y [B, H] in p's type. One launch, nothing allocated but y; for generation: no gradients (a state that requires some is refused)."""
+    -> y [B, H] in p's type. One launch, nothing allocated but y; for generation: no gradients (a state that requires some is refused, and so is a tangent)."""
     hid = _scan_args(p, h, None, out_gate, 2)
+    _runtime.refuse_tangents("gated_scan_step", p, h)
     if h is None or not h.is_contiguous() or h.requires_grad:
         raise ValueError("the state is updated in place: it must be a contiguous tensor that requires no gradient")
     if p.stride(1) != 1:

@@ -309,6 +309,7 @@ def orthogonalize(g, steps=5, eps=1e-7):
         raise ValueError("eps must not be negative, got %r" % (eps,))
     _side_ok(g.shape[-2:], "orthogonalize")
     R.require_here(g)
+    R.refuse_tangents("orthogonalize", g)
     src = g.contiguous()
     out = torch.empty_like(src)
     one = (lambda t: list(t)) if g.dim() == 3 else (lambda t: [t])

@@ -2,6 +2,7 @@
 import os
 
 import torch
+from torch.autograd import forward_ad as _fw
 
 from . import _lib
 
@@ -387,6 +388,12 @@ def require_here(*tensors):
         if at != here:
             require_gpu(t)
             raise RuntimeError("tensor on %s while the current device is cuda:%d: call inside `with torch.cuda.device(...)`" % (t.device, here))
+
+
+def refuse_tangents(what, *tensors):
+    """For calls without an autograd function, whose result would come without a tangent (a zero derivative to forward-mode AD)."""
+    if _fw._current_level >= 0 and any(t is not None and _fw.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("%s has no derivative: the tangent of its input would be lost" % what)
 
 
 def keep_forced(*tensors):

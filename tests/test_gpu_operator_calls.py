@@ -6,6 +6,33 @@ import torch
 pytestmark = pytest.mark.gpu
 
 
+def test_forward_mode_is_refused():
+    """No operator here has a forward-mode derivative: a tangent on any input raises (a result without one would count as a zero
+    derivative). Inputs without tangents give the same bits inside a dual level as outside."""
+    import torch.autograd.forward_ad as fw
+    from cpcsv import functional as F
+    from cpcsv.optim import orthogonalize
+    r = lambda *s: torch.randn(*s, device="cuda")
+    p, h0, x, u, g, w, s, n = r(2, 40, 12), r(2, 4), r(2, 5, 8), r(2, 5, 8), r(2, 1, 8), r(8), r(8), r(8)
+    scan = lambda a, b: F.gated_scan(a, b)[0]
+    norm = lambda *a: F.norm_residual(*a[:3], gate=a[3], scale=a[4], w_next=a[5])[1]
+    step = lambda a, b: F.gated_scan_step(a, b)
+    calls = [(scan, (p, h0)), (norm, (x, u, w, g, s, n)), (F.rms_norm, (x, w)), (step, (p[:, 0], h0.clone())), (orthogonalize, (r(6, 9),))]
+    for f, args in calls:
+        state = args[1].clone() if f is step else None
+        want = f(*args)
+        if f is step:
+            args[1].copy_(state)
+        with fw.dual_level():
+            got = f(*args)
+            assert torch.equal(got, want)
+            for i, t in enumerate(args):
+                dual = fw.make_dual(t.detach(), torch.ones_like(t))
+                for grads in (True, False):
+                    with torch.set_grad_enabled(grads), pytest.raises(NotImplementedError):
+                        f(*args[:i], dual, *args[i + 1:])
+
+
 def dense_error(y, x, w, b, cast):
     """|y - (x w^T + b)| over its bound: operands rounded once to `cast` (half a step each), sums of K products in fp32, y stored in fp32."""
     x, w, b = x.detach().double().cpu(), w.detach().double().cpu(), b.detach().double().cpu()
