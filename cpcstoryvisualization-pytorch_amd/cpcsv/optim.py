@@ -328,7 +328,8 @@ class FusedMuon(torch.optim.Optimizer):
     Up to 16 matrices share each of the 3 steps + 2 launches (csrc/orth.hip); biases, norms and other vectors belong to FusedAdam. Like
     there the learning rate lives on the device (graph replays follow sync_lr()), and parameters, gradients and momentum are contiguous
     fp32 GPU tensors. Operand copies that layers keep of these weights are made anew after a step; once a step has been captured,
-    and inside every graph that a user captures, at each use, since nothing tells the host when a replay has moved the weights."""
+    and inside every graph that a user captures, at each use, since nothing tells the host when a replay has moved the weights.
+    A step counts as an in-place change of the weight: a backward pass that saved it from before is refused."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, eps=1e-7):
         if not lr >= 0 or not 0 <= momentum < 1 or not weight_decay >= 0 or not eps >= 0:
@@ -407,6 +408,8 @@ class FusedMuon(torch.optim.Optimizer):
                 ws = K.muon_step(part, [p.grad for p in part], [self.state[p]["momentum_buffer"] for p in part], [self._matrix(p) for p in part],
                                  hyper, group["momentum"], group["nesterov"], group["weight_decay"], group["steps"], group["eps"])
                 R.keep_forced(ws)
+            # (a graph that saved a weight or its momentum refuses its backward pass; tensors of inference mode have no version)
+            torch.autograd.graph.increment_version([t for p in plist for t in (p, self.state[p]["momentum_buffer"]) if not t.is_inference()])
             for p in plist:      # invalidate packed-operand caches (cpcsv.modules.KernelLayer.packs)
                 p._cpcsv_epoch = getattr(p, "_cpcsv_epoch", 0) + 1
             _note_moves(plist, torch.cuda.is_current_stream_capturing())

@@ -33,6 +33,38 @@ def test_forward_mode_is_refused():
                         f(*args[:i], dual, *args[i + 1:])
 
 
+def test_updated_weights_count_as_modified():
+    """A backward pass through a graph that saved a weight (or the momentum) from before FusedMuon's step is refused, as after torch's own
+    optimisers; a parameter without a gradient is not touched."""
+    from cpcsv.optim import FusedMuon
+    w, still = (torch.nn.Parameter(torch.randn(6, 9, device="cuda")) for _ in range(2))
+    opt = FusedMuon([w, still], lr=0.1)
+    w.grad = torch.randn_like(w)
+    opt.step()
+    m = opt.state[w]["momentum_buffer"]
+    x = torch.randn(9, 3, device="cuda", requires_grad=True)
+    y, z, q = w @ x, (x[:, 0] * m).sum(), still @ x
+    opt.step()
+    for out in (y, z):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()
+    q.sum().backward()
+    assert still._version == 0
+
+
+def test_inference_weights_are_updated():
+    """Tensors made in inference mode have no versions; they are stepped all the same."""
+    from cpcsv.optim import FusedMuon
+    with torch.inference_mode():
+        w = torch.nn.Parameter(torch.ones(6, 9, device="cuda"), requires_grad=False)
+        w.grad = torch.randn(6, 9, device="cuda")
+        opt = FusedMuon([w], lr=0.1)
+        for _ in range(2):
+            before = w.clone()
+            opt.step()
+            assert not torch.equal(w, before)
+
+
 def dense_error(y, x, w, b, cast):
     """|y - (x w^T + b)| over its bound: operands rounded once to `cast` (half a step each), sums of K products in fp32, y stored in fp32."""
     x, w, b = x.detach().double().cpu(), w.detach().double().cpu(), b.detach().double().cpu()
