@@ -171,6 +171,16 @@ struct Look {                        // armed with ones before each use
     unsigned long long* map;         // [B][tiles][H] {A, X}
 };
 struct Map { float a, x; };
+// A product of gates that underflows is not zero: 0 would turn an infinite state into NaN. It stays at fp32's smallest number instead,
+// which adds 2^-149 |h| to a finite state's result: less than 2^-49 for any |h| below 2^100. (A gate that is 0 in fp32, f below about
+// -87, is 0: it makes NaN of an infinite state here as token by token.)
+constexpr float LEAST = 0x1p-149f;
+__device__ __forceinline__ float product(float a, float b) {
+    const float r = a * b;
+    return r == 0.f && a != 0.f && b != 0.f ? LEAST : r;
+}
+// of a chunk, whose gates are multiplied without that test; least: the smallest of them
+__device__ __forceinline__ float whole_product(float a, float least) { return a == 0.f && least > 0.f ? LEAST : a; }
 __device__ __forceinline__ float plain_nan(float v) { return v == v ? v : __uint_as_float(0x7fc00000u); }
 __device__ __forceinline__ void publish(unsigned long long* p, float a, float x) {
     const unsigned long long w = (unsigned long long)__float_as_uint(plain_nan(a)) | (unsigned long long)__float_as_uint(plain_nan(x)) << 32;
@@ -219,7 +229,7 @@ template <int W, int VEC> struct Joint {
                 whole[k] = own[0][at + k];
                 for (int j = 1; j < W; ++j) {
                     const Map m = own[j][at + k];
-                    whole[k] = Map{m.a * whole[k].a, __fmaf_rn(m.a, whole[k].x, m.x)};
+                    whole[k] = Map{product(m.a, whole[k].a), __fmaf_rn(m.a, whole[k].x, m.x)};
                 }
                 if (ok && tile % SB != SB - 1 && tile + 1 < d.NT) publish(maps + (long)tile * d.H + k, whole[k].a, whole[k].x);
             }
@@ -273,9 +283,9 @@ __global__ __launch_bounds__(FW * 64, 4) void scan_fwd_kernel(const T* __restric
     place_of<FW, VEC>(lk, d, sh.ticket, b, tile, ch);
     const bool ok = ch < d.H;
     const int chunk = tile * FW + (threadIdx.x >> 6), t0 = chunk * CH, n = min(max(length_of(d, b) - t0, 0), CH), rows = min(max(d.T - t0, 0), CH);
-    float zs[CH][VEC], in[CH][VEC], act[GATE ? CH : 1][VEC], A[VEC], X[VEC];
+    float zs[CH][VEC], in[CH][VEC], act[GATE ? CH : 1][VEC], A[VEC], X[VEC], least[VEC];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) { A[k] = 1.f; X[k] = 0.f; }
+    for (int k = 0; k < VEC; ++k) { A[k] = least[k] = 1.f; X[k] = 0.f; }
     {
         word<T, VEC> f[CH], v[CH], o[GATE ? CH : 1];
         const T* q = p + b * d.sb + t0 * d.st + (ok ? ch : 0);          // (lanes without channels read the row's first and store nothing)
@@ -301,9 +311,12 @@ __global__ __launch_bounds__(FW * 64, 4) void scan_fwd_kernel(const T* __restric
                     act[i][k] = on ? __fmul_rn(g, gate_of(g).s) : 0.f;
                 }
                 A[k] *= zs[i][k];
+                least[k] = fminf(least[k], zs[i][k]);
                 X[k] = __fmaf_rn(zs[i][k], X[k], in[i][k]);
             }
     }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) A[k] = whole_product(A[k], least[k]);
     float h[VEC];
     sh.enter(lk, d, b, tile, ch, ok, A, X, h0, h);
     if (!ok || !rows) return;
@@ -339,7 +352,7 @@ __global__ __launch_bounds__(BW * 64, 2) void scan_bwd_kernel(const T* __restric
     const bool ok = ch < d.H;
     const int chunk = (d.NT - 1 - tile) * BW + BW - 1 - (int)(threadIdx.x >> 6), t0 = chunk * CH;
     const int n = min(max(length_of(d, b) - t0, 0), CH), rows = ok ? min(max(d.T - t0, 0), CH) : 0;
-    float zs[CH][VEC], zc[CH][VEC], q[CH][VEC], u[CH][VEC], A[VEC], X[VEC];
+    float zs[CH][VEC], zc[CH][VEC], q[CH][VEC], u[CH][VEC], A[VEC], X[VEC], least[VEC];
     const long row0 = (long)b * d.T + t0;
     T* out = dp + row0 * K * d.H + ch;
     {
@@ -383,14 +396,17 @@ __global__ __launch_bounds__(BW * 64, 2) void scan_bwd_kernel(const T* __restric
         }
     }
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) { A[k] = 1.f; X[k] = 0.f; }
+    for (int k = 0; k < VEC; ++k) { A[k] = least[k] = 1.f; X[k] = 0.f; }
 #pragma unroll
     for (int i = CH - 1; i >= 0; --i)
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
             A[k] *= zs[i][k];
+            least[k] = fminf(least[k], zs[i][k]);
             X[k] = zs[i][k] * (X[k] + u[i][k]);
         }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) A[k] = whole_product(A[k], least[k]);
     float C[VEC];
     sh.enter(lk, d, b, tile, ch, ok, A, X, dh_last, C);
     // u of a token behind the end is 0, its z 1: C passes it unchanged, as the map says

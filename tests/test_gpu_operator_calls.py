@@ -198,3 +198,39 @@ def test_eager_layers_follow_replayed_adam_steps(bf16):
         graph.replay()
         assert dense_error(layer(x), x, w, b, torch.float32) <= 1
         assert not torch.equal(w, before)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("t", [20, 100, 700, 1500])
+def test_infinities_stay_infinite(t, dtype):
+    """An infinite state (given, or from an infinite v) or gradient stays infinite however many gates it passes: a product of gates that
+    underflows is still no zero. Where the definition, run token by token, is finite, infinite or NaN, so is the result."""
+    from cpcsv import functional as F
+    g = torch.Generator().manual_seed(t)
+    h = 6
+    p = torch.randn(2, t, 2 * h, generator=g).to(dtype)
+    p[..., :h] -= 3.0                                   # gates about 0.05: sixteen tokens leave 1e-21
+    h0 = torch.randn(2, h, generator=g)
+    h0[0, 0], h0[0, 1], h0[1, 2] = float("inf"), float("-inf"), float("nan")
+    p[0, 3, h + 2], p[1, t // 2, h + 3] = float("inf"), float("-inf")
+    p[1, 1, h + 4], p[1, t - 2, h + 4] = float("inf"), float("-inf")            # meets its opposite: NaN
+    dy, dl = torch.randn(2, t, h, generator=g).to(dtype), torch.randn(2, h, generator=g)
+    dl[0, 5], dl[1, 5], dy[1, t - 4, 0] = float("inf"), float("-inf"), float("inf")
+    z, zc, v = torch.sigmoid(p[..., :h].double()), torch.sigmoid(-p[..., :h].double()), p[..., h:].double()
+    hs, x = [], h0.double()
+    for i in range(t):
+        x = z[:, i] * x + zc[:, i] * v[:, i]
+        hs.append(x)
+    D, dvs = dl.double(), [None] * t
+    for i in range(t - 1, -1, -1):
+        D = D + dy[:, i].double()
+        dvs[i] = D * zc[:, i]
+        D = D * z[:, i]
+    pg, hg = p.cuda().requires_grad_(), h0.cuda().requires_grad_()
+    y, last = F.gated_scan(pg, hg, out_gate=False)
+    dp, dh0 = torch.autograd.grad([y, last], [pg, hg], [dy.cuda(), dl.cuda()])
+    for got, want in ((y, torch.stack(hs, 1)), (last, x), (dp[..., h:], torch.stack(dvs, 1)), (dh0, D)):
+        got = got.detach().cpu().double()
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(torch.isinf(got), torch.isinf(want))
+        assert torch.equal(got[torch.isinf(got)], want[torch.isinf(want)])
