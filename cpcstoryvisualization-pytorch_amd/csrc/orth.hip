@@ -171,12 +171,16 @@ __global__ __launch_bounds__(256) void orth_split_kernel(Jobs s) {
         if (threadIdx.x < o) sh[threadIdx.x] += sh[threadIdx.x + o];
         __syncthreads();
     }
-    const float inv = (float)((double)SX / (sqrt(sh[0]) + (double)s.eps));
+    // u SX / (|U| + eps), the factor as a power of two and the rest: by itself it leaves fp32's range where |U| is tiny (eps 0). Zeros
+    // stay zeros whatever eps is.
+    const double norm = sqrt(sh[0]) + (double)s.eps;
+    int pow2 = 0;
+    const float rest = norm > 0.0 ? (float)frexp((double)SX / norm, &pow2) : norm == 0.0 ? 0.f : (float)norm;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const float v = !j.m ? u[i] : s.nesterov ? __fmaf_rn(s.mu, m[i], u[i]) : m[i];
         const bool in = r0 + i * 4 + rl < j.rows && c < j.cols;
-        t[i * 4 + rl][cl] = split_of(in ? v * inv : 0.f);
+        t[i * 4 + rl][cl] = split_of(in ? ldexpf(v, pow2) * rest : 0.f);
     }
     __syncthreads();
     _Float16 *own = s.ws + (j.tall ? j.xt : j.x), *turned = s.ws + (j.tall ? j.x : j.xt);

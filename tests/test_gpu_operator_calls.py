@@ -234,3 +234,25 @@ def test_infinities_stay_infinite(t, dtype):
         assert torch.equal(torch.isnan(got), torch.isnan(want))
         assert torch.equal(torch.isinf(got), torch.isinf(want))
         assert torch.equal(got[torch.isinf(got)], want[torch.isinf(want)])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_zero_and_tiny_matrices_without_eps(dtype):
+    """eps = 0: a matrix of zeros stays zero, and one whose norm lies below 2^-112 (16384 over it leaves fp32's range), subnormal
+    numbers included, has the direction it has. The scaled matrix holds the same digits, so the results are the same bits."""
+    from cpcsv.optim import FusedMuon, orthogonalize
+    g = torch.randn(70, 90, generator=torch.Generator().manual_seed(4))
+    zero = torch.zeros(70, 90).to(dtype).cuda()
+    assert torch.equal(orthogonalize(zero, eps=0.0), zero)
+    both = orthogonalize(torch.stack([zero, g.to(dtype).cuda()]), eps=0.0)
+    assert torch.equal(both[0], zero) and torch.equal(both[1], orthogonalize(g.to(dtype).cuda(), eps=0.0))
+    g = (g * 64).round().clamp(-127, 127)                # whole numbers of 7 bits: exact in either type at 2^-149 too
+    for e in (-149, -130, -120, -100, 100):
+        small = (g.double() * 2.0 ** e).to(dtype).cuda()
+        if dtype == torch.bfloat16 and e < -133:
+            continue                                     # (below bfloat16's smallest)
+        assert torch.equal(orthogonalize(small, eps=0.0), orthogonalize(g.to(dtype).cuda(), eps=0.0)), e
+    w = torch.nn.Parameter(torch.ones(70, 90, device="cuda"))
+    w.grad = torch.zeros_like(w)
+    FusedMuon([w], lr=0.1, eps=0.0).step()
+    assert torch.equal(w, torch.ones_like(w))
