@@ -361,24 +361,24 @@ class FusedMuon(torch.optim.Optimizer):
         return p.shape[0], (p.numel() // p.shape[0] if p.shape[0] else 0)
 
     def _hyper(self, gi, group, dev):
-        h = self._hypers.get(gi)
+        h, lr = self._hypers.get(gi), float(group["lr"])       # (a tensor may be changed in place: its value is compared)
         if h is None:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("FusedMuon: run one step before capturing one (its device scalars are made there)")
-            h = self._hypers[gi] = [torch.tensor([float(group["lr"])], dtype=torch.float32, device=dev), group["lr"]]
-        elif h[1] != group["lr"]:
+            h = self._hypers[gi] = [torch.tensor([lr], dtype=torch.float32, device=dev), lr]
+        elif h[1] != lr:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("learning rate changed during graph capture")
-            h[0].fill_(float(group["lr"]))
-            h[1] = group["lr"]
+            h[0].fill_(lr)
+            h[1] = lr
         return h[0]
 
     def sync_lr(self):
         """Push host-side lr changes to the device scalars (call after editing param_groups when using HIP graphs)."""
         for gi, group in enumerate(self.param_groups):
-            if gi in self._hypers and self._hypers[gi][1] != group["lr"]:
+            if gi in self._hypers and self._hypers[gi][1] != float(group["lr"]):
                 self._hypers[gi][0].fill_(float(group["lr"]))
-                self._hypers[gi][1] = group["lr"]
+                self._hypers[gi][1] = float(group["lr"])
 
     @torch.no_grad()
     def step(self, closure=None):

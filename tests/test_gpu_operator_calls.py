@@ -256,3 +256,30 @@ def test_zero_and_tiny_matrices_without_eps(dtype):
     w.grad = torch.zeros_like(w)
     FusedMuon([w], lr=0.1, eps=0.0).step()
     assert torch.equal(w, torch.ones_like(w))
+
+
+def test_a_learning_rate_tensor_changed_in_place_is_followed():
+    """lr may be a tensor, which schedulers change in place: each step and sync_lr() read its value."""
+    from cpcsv.optim import FusedMuon
+    gen = torch.Generator("cuda").manual_seed(1)
+    w0, g = torch.randn(30, 40, generator=gen, device="cuda"), torch.randn(30, 40, generator=gen, device="cuda")
+    ends = []
+    for lr in (0.1, torch.tensor(0.1)):
+        w = torch.nn.Parameter(w0.clone())
+        w.grad = g.clone()
+        opt = FusedMuon([w], lr=lr)
+        opt.step()
+        for v in (0.025, 0.5):
+            if torch.is_tensor(lr):
+                lr.fill_(v)
+            else:
+                opt.param_groups[0]["lr"] = v
+            opt.sync_lr()
+            opt.step()
+            if torch.is_tensor(lr):
+                lr.fill_(2 * v)
+            else:
+                opt.param_groups[0]["lr"] = 2 * v
+            opt.step()
+        ends.append(w.detach())
+    assert torch.equal(*ends)
