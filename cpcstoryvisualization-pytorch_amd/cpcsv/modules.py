@@ -599,6 +599,8 @@ class GatedRecurrence(nn.Module):
         """x [..., input_size] -> p [..., 3H or 2H], the input of gated_scan / gated_scan_step."""
         lay = _layer_for(self.proj, None, L.ACT_NONE, 0, out_mode="T")
         rows = x.reshape(-1, self.input_size)
+        if not rows.shape[0]:                      # (no launch for no tokens; the weights' gradients are zeros)
+            return nn.functional.linear(rows.float(), self.proj.master(), self.proj.bias).to(lay.in_dtype()).view(x.shape[:-1] + (self.proj.cout,))
         if rows.dtype != lay.in_dtype() or rows.shape[1] != lay.k_stored:
             rows = rows.float()
         return lay(rows).view(x.shape[:-1] + (pad8(self.proj.cout),))[..., :self.proj.cout]

@@ -283,3 +283,17 @@ def test_a_learning_rate_tensor_changed_in_place_is_followed():
             opt.step()
         ends.append(w.detach())
     assert torch.equal(*ends)
+
+
+@pytest.mark.parametrize("shape", [(0, 4, 8), (2, 0, 8)])
+def test_a_recurrence_over_no_tokens(shape):
+    """GatedRecurrence over an empty batch or empty sequences: as gated_scan, the state passes through; the weights' gradients are zero."""
+    from cpcsv import modules as M
+    for out_gate in (True, False):
+        rec = M.GatedRecurrence(8, 4, out_gate=out_gate).cuda()
+        x, h0 = torch.zeros(shape, device="cuda", requires_grad=True), torch.randn(shape[0], 4, device="cuda", requires_grad=True)
+        y, last = rec(x, h0)
+        assert y.shape == shape[:2] + (4,) and y.dtype == rec(torch.zeros(2, 3, 8, device="cuda"))[0].dtype and torch.equal(last, h0)
+        grads = torch.autograd.grad([y.float().sum() + last.sum()], [x, h0, rec.proj.weight, rec.proj.bias])
+        assert grads[0].shape == shape and torch.equal(grads[1], torch.ones_like(h0)) and not grads[2].any() and not grads[3].any()
+        assert rec.step(torch.zeros(0, 8, device="cuda"), torch.zeros(0, 4, device="cuda")).shape == (0, 4)
