@@ -348,13 +348,20 @@ class FusedMuon(torch.optim.Optimizer):
     def add_param_group(self, group):
         super().add_param_group(group)
         params = self.param_groups[-1]["params"]
+        try:
+            self._check(params)
+        except ValueError:
+            self.param_groups.pop()              # (a refused group is not kept)
+            raise
+        _note_moves(params, False)
+
+    def _check(self, params):
         if len(set(params)) < len(params):
             raise ValueError("FusedMuon: a parameter stands twice in a group (its two updates would run at once)")
         for p in params:
             if p.dim() < 2:
                 raise ValueError("FusedMuon takes matrices (two or more dimensions), got shape %s: leave vectors to FusedAdam" % (tuple(p.shape),))
             _side_ok(self._matrix(p), "FusedMuon")
-        _note_moves(params, False)
 
     @staticmethod
     def _matrix(p):
