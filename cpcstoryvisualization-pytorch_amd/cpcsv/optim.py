@@ -329,6 +329,8 @@ class FusedMuon(torch.optim.Optimizer):
     there the learning rate lives on the device (graph replays follow sync_lr()), and parameters, gradients and momentum are contiguous
     fp32 GPU tensors. Operand copies that layers keep of these weights are made anew after a step; once a step has been captured,
     and inside every graph that a user captures, at each use, since nothing tells the host when a replay has moved the weights.
+    Weights under FusedAdam's deferred layer updates, which GANTrainer sets up for its larger ones, have no gradient to take: they are
+    refused. FusedMuon stands in a training loop of one's own, over cpcsv.modules.
     A step counts as an in-place change of the weight: a backward pass that saved it from before is refused."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, eps=1e-7):
@@ -397,6 +399,9 @@ class FusedMuon(torch.optim.Optimizer):
             plist = [p for p in group["params"] if p.grad is not None]
             for p in plist:
                 st = self.state[p]
+                if getattr(p, "_cpcsv_retired", False):
+                    raise RuntimeError("FusedMuon: a weight of shape %s is under the deferred update of its layer (FusedAdam.attach_layer, as "
+                                       "GANTrainer sets it up): its gradient never leaves the layer's accumulator" % (tuple(p.shape),))
                 ok = lambda t: t.is_cuda and t.dtype == torch.float32 and t.is_contiguous() and t.shape == p.shape
                 if not ok(p) or not ok(p.grad):
                     raise RuntimeError("FusedMuon needs contiguous fp32 GPU parameters and gradients")

@@ -16,3 +16,13 @@ def test_a_refused_group_is_not_kept():
     assert len(opt.param_groups) == 1
     opt.add_param_group({"params": [other], "lr": 0.1})              # (free to join: the refused groups left no trace)
     assert len(opt.param_groups) == 2 and opt.state_dict()["param_groups"][1]["lr"] == 0.1
+
+
+def test_weights_of_a_deferred_update_are_named():
+    """GANTrainer's larger weights have no gradient of their own (FusedAdam.attach_layer: it stays in the layer's accumulator)."""
+    from cpcsv.dist import GradBucket
+    from cpcsv.optim import FusedMuon
+    w = torch.nn.Parameter(torch.zeros(4, 6))
+    GradBucket([w, torch.nn.Parameter(torch.zeros(3))]).adopt(retired=[w])
+    with pytest.raises(RuntimeError, match="deferred update"):
+        FusedMuon([w]).step()
