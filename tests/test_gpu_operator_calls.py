@@ -297,3 +297,28 @@ def test_a_recurrence_over_no_tokens(shape):
         grads = torch.autograd.grad([y.float().sum() + last.sum()], [x, h0, rec.proj.weight, rec.proj.bias])
         assert grads[0].shape == shape and torch.equal(grads[1], torch.ones_like(h0)) and not grads[2].any() and not grads[3].any()
         assert rec.step(torch.zeros(0, 8, device="cuda"), torch.zeros(0, 4, device="cuda")).shape == (0, 4)
+
+
+@pytest.mark.parametrize("d,h", [(40, 48), (365, 100)])
+def test_the_documented_block_runs(d, h, bf16):
+    """The documents' example as it is printed, then a step of its optimisers."""
+    import glob
+    import os
+    import re
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    blocks = [b for f in glob.glob(os.path.join(root, "*.md")) for b in re.findall(r"```python\n(.*?)```", open(f).read(), re.S) if "GatedRecurrence(" in b]
+    assert blocks
+    for text in blocks:
+        from cpcsv import functional, modules, runtime
+        x, x_t = torch.randn(3, 7, d, device="cuda"), torch.randn(3, d, device="cuda")
+        names = dict(torch=torch, M=modules, F=functional, runtime=runtime, d=d, h=h, x=x, x_t=x_t,
+                     lengths=torch.tensor([7, 0, 3], dtype=torch.int32, device="cuda"))
+        exec(text, names)
+        assert names["y_t"].shape == (3, h) and names["z"].shape == x.shape
+        (names["x1"].sum() + names["z"].square().sum()).backward()
+        held = [p for m in ("norm", "rec", "out", "post") for p in names[m].parameters()]
+        before = [p.detach().clone() for p in held]
+        assert sorted(id(p) for o in names["opt"] for g in o.param_groups for p in g["params"]) == sorted(id(p) for p in held)
+        for o in names["opt"]:
+            o.step()
+        assert all(torch.isfinite(p).all() and not torch.equal(p, q) for p, q in zip(held, before))
