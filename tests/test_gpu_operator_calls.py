@@ -236,6 +236,17 @@ def test_infinities_stay_infinite(t, dtype):
         assert torch.equal(got[torch.isinf(got)], want[torch.isinf(want)])
 
 
+@pytest.mark.parametrize("dtype,h", [(torch.bfloat16, 512), (torch.float32, 250)])
+def test_more_blocks_than_the_chip_holds(dtype, h):
+    """One call of over a thousand blocks forward and two thousand backward (512 of either fit), 17 and 33 tiles a row: blocks start when
+    others retire, states pass several runs of tiles. Against the recurrence in 64 bits, with the bounds of the recurrence's own tests."""
+    from tests.test_gpu_scan import check, make
+    b, t = 16, 2100
+    groups = -(-h // (128 if dtype == torch.bfloat16 else 64))
+    assert -(-t // 128) * b * groups > 1024 and -(-t // 64) * b * groups > 2048
+    check(*make(b, t, h, True, dtype, seed=11, lengths=[t, 1, 0, 2049, 2048, 1025, 130] + [t - 64 * i for i in range(9)]), True)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_zero_and_tiny_matrices_without_eps(dtype):
     """eps = 0: a matrix of zeros stays zero, and one whose norm lies below 2^-112 (16384 over it leaves fp32's range), subnormal
