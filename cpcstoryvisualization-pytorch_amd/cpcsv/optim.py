@@ -397,6 +397,9 @@ class FusedMuon(torch.optim.Optimizer):
                 loss = closure()
         for gi, group in enumerate(self.param_groups):
             plist = [p for p in group["params"] if p.grad is not None]
+            spans = sorted((p.data_ptr(), p.numel() * p.element_size()) for p in plist)
+            if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])):
+                raise RuntimeError("FusedMuon: two parameters of a group share memory (their updates would run at once)")
             for p in plist:
                 st = self.state[p]
                 if getattr(p, "_cpcsv_retired", False):

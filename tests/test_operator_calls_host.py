@@ -26,3 +26,24 @@ def test_weights_of_a_deferred_update_are_named():
     GradBucket([w, torch.nn.Parameter(torch.zeros(3))]).adopt(retired=[w])
     with pytest.raises(RuntimeError, match="deferred update"):
         FusedMuon([w]).step()
+
+
+def test_weights_that_share_memory_are_refused():
+    """Matrices of a group are updated at once: two that overlap (a tied weight held twice, a slice of another) would race. Neighbours in
+    one buffer do not overlap."""
+    from cpcsv.optim import FusedMuon
+    base = torch.zeros(10, 6)
+    held = lambda *views: [torch.nn.Parameter(v) for v in views]
+    for params in (held(base, base), held(base, base[3:5]), held(base[4:], base[:5])):
+        for p in params:
+            p.grad = torch.zeros_like(p)
+        with pytest.raises(RuntimeError, match="share memory"):
+            FusedMuon(params).step()
+        params[1].grad = None                                        # (only one of them moves)
+        with pytest.raises(RuntimeError, match="contiguous fp32 GPU"):
+            FusedMuon(params).step()
+    apart = held(base[5:], base[:5])
+    for p in apart:
+        p.grad = torch.zeros_like(p)
+    with pytest.raises(RuntimeError, match="contiguous fp32 GPU"):
+        FusedMuon(apart).step()
