@@ -1592,7 +1592,8 @@ def _norm_x(x):
 
 
 def rms_norm(x, weight, eps=1e-6, out_dtype=None):
-    """weight * x / sqrt(mean x^2 + eps) over the last dimension (fp32 or bf16 x, fp32 weight [D], D <= 16384), statistics in fp32.
+    """weight * x / sqrt(mean x^2 + eps) over the last dimension (fp32 or bf16 x, fp32 weight [D], D <= 16384), statistics in fp32
+    (squares of entries above about 1e17 leave its range, and with eps = 0 those of rows below 1e-19).
     out_dtype: the result's type (default x's; bf16 from an fp32 residual stream feeds the compute dtype). The norm before the first
     block; norm_residual holds those behind it."""
     d = _norm_x(x)

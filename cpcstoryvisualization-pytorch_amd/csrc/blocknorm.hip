@@ -4,12 +4,19 @@
 // (u the block's output, x the residual stream, z the next block's input), and their gradients. With g = dz w_next:
 //     dx = dx' + rx (g - xh mean(g xh))             q = dx scale gate w_post       du = ru (q - uh mean(q uh))
 //     dgate = dx scale w_post uh    dw_next = sum dz xh    dw_post = scale sum(dx gate uh)    dscale = w_post sum(dx gate uh)
-// HBM-bound: every tensor is read or written once. x' is formed again in the backward pass from x and u (the same bytes as reading
+// HBM-bound: every tensor is read or written once (but for spilled registers, below). x' is formed again in the backward pass from x and u (the same bytes as reading
 // it, and exactly the forward's fp32 value rather than its rounded copy), the row statistics are two floats a row.
-// A row is owned by `tpr` threads (64: one wavefront, no barrier; up to 1024 for wide rows) that keep 8 values each in registers
-// between the two reductions, with their share of the weights beside them: blocks walk many rows, so the weights are read once a
-// block, and the next row is loaded before this one's reductions. 32768 rows of 2048 in bf16 with a gate a token: forward 135 us,
-// 5.0 TB/s; backward 224 us, 4.8 TB/s (a large copy: 4.9 to 5.4). 8192 rows of 8192, an fp32 stream: 182 and 289 us, 4.4 and 4.2 TB/s.
+// A row is owned by `tpr` threads (64: one wavefront, no barrier; up to 1024 for wide rows) that keep 8 values each (16 above 8192
+// columns) in registers between the two reductions, with their share of the weights beside them: blocks walk many rows, so the weights
+// are read once a block, and the next row is loaded before this one's reductions. 32768 rows of 2048 in bf16 with a gate a token:
+// forward 135 us, 5.0 TB/s; backward 224 us, 4.8 TB/s (a large copy: 4.9 to 5.4). 8192 rows of 8192, an fp32 stream: 182 and 289 us,
+// 4.4 and 4.2 TB/s.
+// One bound of 1024 threads a block serves all widths: 128 registers, and the backward kernel needs more. Only its 16-byte bf16 form of
+// 8 values has no scratch; bytes a lane elsewhere: 16-byte rows up to 8192 columns 28 (fp32 stream, bf16 branch) and 120 (all fp32), odd
+// rows 64 to 132, rows above 8192 columns 188 to 308, odd ones 632 to 744 (their forward 8 to 72). What that costs, both ways, no gate,
+// against the bytes at 5.0 TB/s: 32768 x 2048 in fp32 583 us and 537; 12276 x 365 53 to 65 and 18 to 36 (value-by-value loads too);
+// 8192 x 12288 1080 to 1490 and 400 to 810; 8192 x 16384 1260 to 1750 and 540 to 1070; 2048 x 16383 860 to 960 and 130 to 270.
+// Squares are summed in fp32: entries above about 1e17 leave its range (1/rms becomes 0), as do rows below 1e-19 if eps is 0.
 // The weight gradients' column sums accumulate in registers over a block's rows and are joined by a second launch (8 us) in a fixed
 // order.
 #include "common.h"

@@ -2,7 +2,8 @@
 //     m <- mu m + g      U = g + mu m (nesterov) or m      X = U / (|U|_F + eps)
 //     five times   X <- P(X X^T) X,  P(A) = a I + b A + c A^2          w <- w (1 - lr decay) - lr sqrt(max(1, rows / cols)) X
 // with (a, b, c) the quintic whose iteration takes singular values of (0, 1] towards 1; a tall matrix is worked on transposed, so
-// that A is the smaller (M x M) Gram matrix.
+// that A is the smaller (M x M) Gram matrix. The coefficients, the momentum rule and the scale of the update are those of the published
+// Muon method (K. Jordan and others, 2024).
 //
 // Through the Gram matrix. Everything an iteration applies to X is a polynomial of A, and the next Gram matrix is P A P: up to three
 // iterations run on M x M matrices alone (Q <- P Q collects what they apply, A <- P (P A)), then X <- Q X once. Five iterations in
@@ -13,9 +14,11 @@
 //
 // Precision. One product in bf16 per step leaves the result 1e-2 off on well conditioned gradients and 3e-1 on those with a few
 // strong directions: what is lost next to the large singular values is amplified by a^5 = 485 where they are small. The operands
-// are therefore kept as TWO fp16 planes each, v = hi + lo with hi = fp16(v), lo = fp16(v - hi): 22 bits and lo's sign, an fp32's
-// accuracy. A product is three MFMAs (hi hi, hi lo, lo hi; lo lo lies below the planes' own rounding), accumulated in fp32. The
-// planes are scaled by powers of two so that entries far below 1 keep their low bits above fp16's subnormal step.
+// are therefore kept as TWO fp16 planes each, v = hi + lo with hi = fp16(v), lo = fp16(v - hi): 22 bits and lo's sign for fp32's
+// 24. A product is three MFMAs (hi hi, hi lo, lo hi; lo lo lies below the planes' own rounding), accumulated in fp32. The planes are
+// scaled by powers of two so that entries far below 1 keep their low bits above fp16's subnormal step. Off the 64-bit result, beside
+// the same five iterations in fp32 (gradients with four strong directions): 63 x 124 2.9e-6 and 1.4e-6, 128 x 128 2.1e-6 and 1.4e-6,
+// 248 x 1780 2.7e-6 and 2.1e-6, 372 x 372 to 1024 x 1024 the same, 1024 x 18432 1.4e-6 and 4.1e-6, 4096 x 4096 6.5e-6 and 4.8e-6.
 //
 // All matrices of a call share each launch (a task list by value, no device tables): the products of one dependency level. Planes
 // are padded to whole tiles with zeros, which stay zeros, so that the K loops have no bounds.

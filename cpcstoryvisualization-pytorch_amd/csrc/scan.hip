@@ -15,8 +15,9 @@
 // by induction over the counter, its state), so every wait ends. A published word is its own flag: 64 (state: 32) bits written and
 // read as one, all ones until then; a NaN is published as another pattern.
 // Bound by HBM: p, y (dy, dp) once each. 8 x 4096 x 2048 in bf16 (a large copy: 4.9 to 5.4 TB/s): forward 127 us, 4.2 TB/s; backward
-// 209 us, 4.5 TB/s; one sequence of 32768 x 2048: 127 us. Two launches (the words are armed first, 2 to 5 us); T <= SHORT runs as one,
-// from start to end in registers, bit for bit what single tokens give (64 x 512, one token: 3 us).
+// 209 us, 4.5 TB/s; one sequence of 32768 x 2048: 128 us (fp32: 198 us, 5.4 TB/s). Two launches (the words are armed first, 2 to 5 us); T <= SHORT runs as one,
+// from start to end in registers, bit for bit what single tokens give (64 x 512, one token: 3 us; 12 x 5 x 365 in fp32: 6 us, both ways
+// 12; 64 x 32 x 2048 in bf16: 17 and 41 us for bytes of 7 and 19 at 5.0 TB/s - one thread walks the sequence, latency).
 #include "common.h"
 #include "../../include/cpcsv_hip.h"
 

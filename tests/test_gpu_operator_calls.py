@@ -269,6 +269,21 @@ def test_zero_and_tiny_matrices_without_eps(dtype):
     assert torch.equal(w, torch.ones_like(w))
 
 
+@pytest.mark.parametrize("rows,cols", [(63, 124), (500, 130), (992, 7936)])
+def test_16_bit_results_are_the_fp32_results_rounded(rows, cols):
+    """A bf16 gradient gives the fp32 call's result of the same numbers, rounded once: where it differs from another form's result, that
+    form's fp32 value lay on the other side of a rounding border. Repeated with other matrices in between, the same bits."""
+    from cpcsv.optim import orthogonalize
+    gen = torch.Generator("cuda").manual_seed(rows)
+    g, other = ((torch.randn(rows, cols, generator=gen, device="cuda") + torch.randn(rows, 4, generator=gen, device="cuda") @ torch.randn(
+        4, cols, generator=gen, device="cuda")).bfloat16() for _ in range(2))
+    got = orthogonalize(g)
+    assert torch.equal(got, orthogonalize(g.float()).bfloat16())
+    for _ in range(5):
+        orthogonalize(other)
+        assert torch.equal(orthogonalize(g), got)
+
+
 def test_a_learning_rate_tensor_changed_in_place_is_followed():
     """lr may be a tensor, which schedulers change in place: each step and sync_lr() read its value."""
     from cpcsv.optim import FusedMuon
