@@ -325,12 +325,12 @@ class FusedMuon(torch.optim.Optimizer):
     """Momentum, orthogonalised: for weights that act as matrices (dense, convolution - seen as [out, inputs x taps] -, recurrent).
         m <- momentum m + g;  U = g + momentum m (nesterov) or m;  X = orthogonalize(U);
         w <- w (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) X
-    Up to 16 matrices share each launch (csrc/orth.hip): two, and the dependent levels of the products, 10 for a run of three iterations, 7
-    for one of two, 3 for one (five steps: 17); a level may take one more for its larger tiles and one that adds up slices. Biases, norms
-    and other vectors belong to FusedAdam. Like there the learning rate lives on the device (graph replays follow sync_lr()), and
+    Up to 16 matrices share each launch (csrc/orth.hip): two, and the dependent levels of the products (five steps: 15, or 17 where wide
+    matrices are among them); a level may take one more for its larger tiles and one that adds up slices. Biases, norms and other
+    vectors belong to FusedAdam. Like there the learning rate lives on the device (graph replays follow sync_lr()), and
     parameters, gradients and momentum are contiguous fp32 GPU tensors. Operand copies that layers keep of these weights are made anew
     after a step; once a step has been captured, and inside every graph that a user captures, at each use, since nothing tells the
-    host when a replay has moved the weights. Working memory of a call: 3.6 (wide) to 9.5 (square) times the matrices' bytes.
+    host when a replay has moved the weights. Working memory of a call: 3.6 (wide) to 6 times the matrices' bytes.
     Weights under FusedAdam's deferred layer updates, which GANTrainer sets up for its larger ones, have no gradient to take: they are
     refused. FusedMuon stands in a training loop of one's own, over cpcsv.modules.
     A step counts as an in-place change of the weight: a backward pass that saved it from before is refused."""

@@ -8,20 +8,22 @@
 // Through the Gram matrix. Everything an iteration applies to X is a polynomial of A, and the next Gram matrix is P A P: up to three
 // iterations run on M x M matrices alone (Q <- P Q collects what they apply, A <- P (P A)), then X <- Q X once. Five iterations in
 // two runs (3 + 2) cost 6 M^2 N + 14 M^3 instead of the 15 M^2 N + 5 M^3 of forming X each time (all M x M results are symmetric:
-// one triangle is computed): equal for square matrices, 2.5 times fewer operations for wide ones. Runs longer than three lose what
-// lies far below the largest singular value (the Gram matrix holds its square): in fp32 all five in one run are up to 25 times
-// further off than X formed each time, 3 + 2 at most twice.
+// one triangle is computed): equal for square matrices, 2.5 times fewer operations for wide ones. But the Gram matrix holds squares, and
+// what is rounded off beside the largest is amplified with the smallest: in fp32 all five in one run are up to 25 times further off than
+// X formed each time, 3 + 2 at most twice. Runs of three are for matrices that are wide enough to gain by them (run_of).
 //
 // Precision. One product in bf16 per step leaves the result 1e-2 off on well conditioned gradients and 3e-1 on those with a few
 // strong directions: what is lost next to the large singular values is amplified by a^5 = 485 where they are small. The operands
 // are therefore kept as TWO fp16 planes each, v = hi + lo with hi = fp16(v), lo = fp16(v - hi): 22 bits and lo's sign for fp32's
 // 24. A product is three MFMAs (hi hi, hi lo, lo hi; lo lo lies below the planes' own rounding), accumulated in fp32. The planes are
 // scaled by powers of two so that entries far below 1 keep their low bits above fp16's subnormal step. Off the 64-bit result, beside
-// the same five iterations in fp32 (gradients with four strong directions): 63 x 124 2.9e-6 and 1.4e-6, 128 x 128 2.1e-6 and 1.4e-6,
-// 248 x 1780 2.7e-6 and 2.1e-6, 372 x 372 to 1024 x 1024 the same, 1024 x 18432 1.4e-6 and 4.1e-6, 4096 x 4096 6.5e-6 and 4.8e-6.
+// the same five iterations in fp32 (gradients with four strong directions): 63 x 124 1.2e-6 and 1.4e-6, 128 x 128 0.7e-6 and 1.4e-6,
+// 372 x 372 0.9e-6 and 2.0e-6, 4096 x 4096 3.3e-6 and 4.8e-6; in runs of three 248 x 1780 2.7e-6 and 2.1e-6, 1095 x 465 2.6e-6 and 2.9e-6,
+// 1024 x 18432 1.4e-6 and 4.1e-6. Matrices of 16 to 32 with strong directions alone 3.5e-6 and 2.6e-6.
 //
-// All matrices of a call share each launch (a task list by value, no device tables): the products of one dependency level. Planes
-// are padded to whole tiles with zeros, which stay zeros, so that the K loops have no bounds.
+// All matrices of a call share each launch (a task list by value, no device tables): the products of one dependency level, of matrices
+// with short and with long runs alike. Planes are padded to whole tiles with zeros, which stay zeros, so that the K loops have no
+// bounds.
 #include "common.h"
 #include "../../include/cpcsv_hip.h"
 #include <algorithm>
@@ -37,7 +39,7 @@ constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 // values stay below fp16's 65504.
 constexpr float SX = 16384.f, SA = 16384.f, SP = 8192.f;
 constexpr float SQ[4] = {0.f, SP, 4096.f, 1024.f};
-constexpr int RUN = 3;                         // iterations between two X
+constexpr int RUN = 3;                         // most iterations between two X
 constexpr int PAD = 128, MAXJ = CPCSV_ORTH_JOBS, MAXT = 2 * MAXJ, NORMB = 1024;      // NORMB: most blocks of a matrix' norm
 
 struct Job {
@@ -45,6 +47,7 @@ struct Job {
     long x, xt;                               // offsets in halves
     int rows, cols;                           // of the matrix
     int M, N, tall;                           // padded min / max side; tall: rows > cols
+    int run;                                  // iterations between two X
     int t_norm, t_split;                      // first block of the job
 };
 struct Jobs {
@@ -207,7 +210,8 @@ __global__ __launch_bounds__(256) void orth_split_kernel(Jobs s) {
 // ---- the products: D = alpha P Q^T + beta E + gamma I over two-plane operands [rows][K] ------------------------------
 // D symmetric, lower triangle and its mirror image (SYMM_E: with E and I) | D and its transpose | the result | the weight. A launch has
 // one kind and its own kernel: straight-line code for all of them was 68 KB, and what a block runs once comes cold from memory
-enum { SYMM, SYMM_E, BOTH, OUT, WEIGHT };
+// (MIXED: products of the first and the third kind, where jobs of short and of long runs share a call)
+enum { SYMM, SYMM_E, BOTH, OUT, WEIGHT, MIXED };
 __host__ __device__ constexpr bool symmetric(int kind) { return kind == SYMM || kind == SYMM_E; }
 struct Task {
     long p, q, e, d, dt;       // offsets in halves; OUT, WEIGHT: d is the output's address
@@ -217,7 +221,10 @@ struct Task {
     int shape, t0, tiles, whole, S, r0; // tile shape; first block; tiles, of which `whole` in one piece, the others in S slices of K; first joining block
     int steps, longer;         // K steps of a slice; slices that have one more
     int rows, cols, tall;                     // OUT, WEIGHT: of the output
+    int symm;
 };
+constexpr bool result(int kind) { return kind == OUT || kind == WEIGHT; }
+template <int KIND> __device__ __forceinline__ bool symm_of(const Task& t) { return KIND == MIXED ? t.symm != 0 : symmetric(KIND); }
 struct Launch {
     int first[MAXT];           // block of each task (behind the last: none's)
     Task t[MAXT];
@@ -262,7 +269,7 @@ __device__ __forceinline__ unsigned triangle_row(unsigned w) {
 }
 template <int KIND> __device__ __forceinline__ void tile_of(const Task& t, unsigned tile, unsigned bm, int& ti, int& tj) {
     const unsigned tm = (t.R + bm - 1) / bm;
-    if (symmetric(KIND)) {
+    if (symm_of<KIND>(t)) {
         // lower triangle by blocks of g x g tiles, a row of blocks behind the other (the last one of h tile rows; on the diagonal
         // triangles): a run of tiles shares operand rows in L2. Row by row, every XCD read the whole operand.
         const unsigned lg = tm >= 24 ? 3 : 2, g = 1u << lg;
@@ -312,7 +319,7 @@ __device__ __forceinline__ void to_lds(const Launch& s, const Task& t, int r0, i
             for (int j = 0; j < 4; ++j) {
                 float v = acc[b][g * 4 + j] * t.alpha;
                 if (KIND == SYMM_E) v += ((float)q.hi[j] + (float)q.lo[j]) * t.beta + (r + j == c ? t.gamma : 0.f);
-                buf[(rl + j) * (C::SW + 1) + cl] = KIND >= OUT ? __float_as_uint(v) : split_of(v);
+                buf[(rl + j) * (C::SW + 1) + cl] = result(KIND) ? __float_as_uint(v) : split_of(v);
             }
         }
 }
@@ -339,7 +346,7 @@ template <typename C, int KIND>
 __device__ __forceinline__ void leave(const Launch& s, const Task& t, int r0, int c0, const uint32_t* buf) {
     constexpr int SW = C::SW, LDW = SW + 1, NB = C::NB;
     const int lane = threadIdx.x & 63;
-    if (KIND >= OUT) {
+    if (result(KIND)) {
         // rows of the output run along the strip's columns, of a tall one's along its rows; GO rows at a time are read before they are
         // written (the weight's: one after the other they cost a memory latency each)
         constexpr int GO = 16;
@@ -368,11 +375,11 @@ __device__ __forceinline__ void leave(const Launch& s, const Task& t, int r0, in
         }
         return;
     }
-    _Float16 *const d = s.ws + t.d, *const turned = s.ws + (symmetric(KIND) ? t.d : t.dt);             // (D^T [C][R])
+    _Float16 *const d = s.ws + t.d, *const turned = s.ws + (symm_of<KIND>(t) ? t.d : t.dt);             // (D^T [C][R])
     for (int b = 0; b < NB; ++b) {
         const int cb = c0 + b * 32;
-        if (symmetric(KIND) && cb > r0) continue;              // (above the diagonal)
-        if (symmetric(KIND) && cb == r0) {
+        if (symm_of<KIND>(t) && cb > r0) continue;             // (above the diagonal)
+        if (symm_of<KIND>(t) && cb == r0) {
             // on it: each pair of entries is taken from the lower one (the two sums are the same numbers in another order)
             block_out<C, MIRRORED>(buf + b * 32, d, r0, cb, t.C);
             continue;
@@ -388,7 +395,7 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 // (sides are multiples of a strip's)
-template <int KIND> __device__ __forceinline__ bool outside(const Task& t, int r0, int c0) { return r0 >= t.R || c0 >= t.C || (symmetric(KIND) && r0 + 31 < c0); }
+template <int KIND> __device__ __forceinline__ bool outside(const Task& t, int r0, int c0) { return r0 >= t.R || c0 >= t.C || (symm_of<KIND>(t) && r0 + 31 < c0); }
 
 // all but the N youngest loads have landed, the wavefront's LDS reads are done
 template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
@@ -658,12 +665,19 @@ Cut cut_of(int kind, long R, long C, long K) {
     return best;
 }
 
+// Iterations between two X of a matrix, by its own (padded) sides: runs on the Gram matrix where they save work. At M x (M + 512) the
+// two ways take the same time (1024 x 1536 213 us either way; runs of one and of three: 1024 x 1024 175 and 198, 1024 x 2048 241 and
+// 225, 4096 x 4096 3825 and 4070, 128 x 512 99 and 106, 128 x 2048 118 and 112). Up to 16 rows or columns X is formed each time
+// however long the other side is: a few strong directions are most of such a matrix, and runs of three lose in accuracy (16 x 2048 2.1
+// times fp32's distance from the 64-bit result, against 1.4; 117 us against 112).
+int run_of(const Job& j) { return j.N - j.M <= 512 || min(j.rows, j.cols) <= 16 ? 1 : RUN; }
+
 struct Plan { long planes, slabs, bytes; int norm, split; };
 struct Scratch { long a, p0, p1, r, q0, q1, xt1; };          // M x M matrices of a job and the second X^T
 
 int plan(Jobs& s, Scratch* sc, const long* dims, int njobs, Plan& p) {
     if (njobs <= 0 || njobs > MAXJ || !dims) return -1001;
-    long at = 0, gram = 0, small = 0, apply = 0;
+    long at = 0, slabs = 0;
     p = Plan{0, 0, 0, 0, 0};
     for (int i = 0; i < njobs; ++i) {
         const long r = dims[2 * i], c = dims[2 * i + 1];
@@ -672,21 +686,20 @@ int plan(Jobs& s, Scratch* sc, const long* dims, int njobs, Plan& p) {
         j.rows = (int)r; j.cols = (int)c; j.tall = r > c;
         j.M = (int)((j.tall ? c : r) + PAD - 1) / PAD * PAD;
         j.N = (int)((j.tall ? r : c) + PAD - 1) / PAD * PAD;
+        j.run = run_of(j);
         const long mn = 2L * j.M * j.N, mm = 2L * j.M * j.M;
         j.x = at; j.xt = at + mn; sc[i].xt1 = at + 2 * mn;
         at += 3 * mn;
         long* const m6[6] = {&sc[i].a, &sc[i].p0, &sc[i].p1, &sc[i].r, &sc[i].q0, &sc[i].q1};
-        for (long* v : m6) { *v = at; at += mm; }
+        for (int k = 0; k < (j.run == 1 ? 2 : 6); ++k) { *m6[k] = at; at += mm; }
         j.t_norm = p.norm; j.t_split = p.split;
         p.norm += norm_blocks(j.rows, j.cols);
         const long t64 = (long)(j.M / 64) * (j.N / 64);
         if (p.split + t64 > (1L << 30)) return -1002;
         p.split += (int)t64;
-        gram += cut_of(SYMM, j.M, j.M, j.N).slab;               // (a level holds one product of a job, two of its M x M ones)
-        small += 2 * cut_of(SYMM, j.M, j.M, j.M).slab;
-        apply += cut_of(BOTH, j.M, j.N, j.M).slab;
+        // (a level holds one product of a job, two of its M x M ones)
+        slabs += max(max(cut_of(SYMM, j.M, j.M, j.N).slab, 2 * cut_of(SYMM, j.M, j.M, j.M).slab), cut_of(BOTH, j.M, j.N, j.M).slab);
     }
-    const long slabs = max(gram, max(small, apply));
     s.n = njobs;
     p.planes = at;
     p.slabs = slabs;
@@ -713,9 +726,10 @@ int run_level(const Launch& all, long slabs, hipStream_t st) {
     long at = 0, units[2] = {0, 0}, joins = 0;
     for (int i = 0; i < all.n; ++i) {
         Task t = all.t[i];
-        const Cut cut = cut_of(all.kind, t.R, t.C, t.K);
+        const int kind = all.kind != MIXED ? all.kind : t.symm ? SYMM : BOTH;
+        const Cut cut = cut_of(kind, t.R, t.C, t.K);
         t.shape = cut.shape;
-        t.tiles = (int)tiles_of(all.kind, t.R, t.C, SHAPES[cut.shape].bm);
+        t.tiles = (int)tiles_of(kind, t.R, t.C, SHAPES[cut.shape].bm);
         t.whole = cut.whole; t.S = cut.S; t.slab = at;
         t.steps = t.K / SHAPES[cut.shape].bk / t.S; t.longer = t.K / SHAPES[cut.shape].bk % t.S;
         at += cut.slab;
@@ -733,6 +747,7 @@ int run_level(const Launch& all, long slabs, hipStream_t st) {
         case SYMM: return fire<SYMM>(big, rest, join, units[0], units[1], joins, st);
         case SYMM_E: return fire<SYMM_E>(big, rest, join, units[0], units[1], joins, st);
         case BOTH: return fire<BOTH>(big, rest, join, units[0], units[1], joins, st);
+        case MIXED: return fire<MIXED>(big, rest, join, units[0], units[1], joins, st);
         case OUT: return fire<OUT>(big, rest, join, units[0], units[1], joins, st);
         default: return fire<WEIGHT>(big, rest, join, units[0], units[1], joins, st);
     }
@@ -749,39 +764,72 @@ int iterate(Jobs& s, const Scratch* sc, const Plan& p, int steps, const float* h
     auto add = [&](int kind, const Job& j, long pp, long q, long d, int C, int K, float alpha) -> Task& {
         Task& t = L.t[L.n++];
         t = Task{};
-        t.p = pp; t.q = q; t.d = d; t.R = j.M; t.C = C; t.K = K; t.alpha = alpha;
-        L.kind = kind;
+        t.p = pp; t.q = q; t.d = d; t.R = j.M; t.C = C; t.K = K; t.alpha = alpha; t.symm = symmetric(kind);
         return t;
     };
-    auto level = [&]() { const int rc = run_level(L, p.slabs, st); L.n = 0; return rc; };
-#define LEVEL(...)                                                          \
-    do {                                                                    \
-        for (int i = 0; i < s.n; ++i) { const Job& j = s.j[i]; const Scratch& c = sc[i]; __VA_ARGS__ } \
-        if (int rc = level()) return rc;                                    \
-    } while (0)
-    bool odd = false;                            // which X^T is current
-    for (int done = 0; done < steps;) {
-        const int run = min(RUN, steps - done);
-        LEVEL(add(SYMM, j, j.x, j.x, c.a, j.M, j.N, SA / (SX * SX)););
-        for (int k = 1; k <= run; ++k) {
-            // P_k in p0, p1 in turn; Q_1 = P_1, Q_2 = P_2 P_1 in q0, Q_3 = P_3 Q_2 in q1
-            LEVEL(Task& t = add(SYMM_E, j, c.a, c.a, k & 1 ? c.p0 : c.p1, j.M, j.M, NS_C * SP / (SA * SA));
-                  t.e = c.a; t.beta = NS_B * SP / SA; t.gamma = NS_A * SP;);
-            if (k > 1 || k < run)
-                LEVEL(const long pk = k & 1 ? c.p0 : c.p1;
-                      if (k < run) add(SYMM, j, pk, c.a, c.r, j.M, j.M, 1.f / SP);
-                      if (k > 1) add(SYMM, j, pk, k == 2 ? c.p0 : c.q0, k == 2 ? c.q0 : c.q1, j.M, j.M, SQ[k] / (SP * SQ[k - 1])););
-            if (k < run) LEVEL(add(SYMM, j, k & 1 ? c.p0 : c.p1, c.r, c.a, j.M, j.M, 1.f / SP););
+    // where a job stands. P_k in p0, p1 in turn; Q_1 = P_1, Q_2 = P_2 P_1 in q0, Q_3 = P_3 Q_2 in q1
+    enum { GRAM, POLY, COLLECT, NEXT, APPLY, END };
+    struct { int phase, done, run, k; bool odd; } at[MAXJ] = {};               // odd: which X^T is current
+    auto kind_of = [&](int i) {
+        const auto& w = at[i];
+        return w.phase == END ? -1 : w.phase == POLY ? SYMM_E : w.phase != APPLY ? SYMM : w.done + w.run < steps ? BOTH : hyper ? WEIGHT : OUT;
+    };
+    auto emit = [&](int i) {
+        const Job& j = s.j[i];
+        const Scratch& c = sc[i];
+        auto& w = at[i];
+        const long pk = w.k & 1 ? c.p0 : c.p1;
+        switch (w.phase) {
+            case GRAM:
+                w.run = min(j.run, steps - w.done);
+                w.k = 1;
+                add(SYMM, j, j.x, j.x, c.a, j.M, j.N, SA / (SX * SX));
+                w.phase = POLY;
+                return;
+            case POLY: {
+                Task& t = add(SYMM_E, j, c.a, c.a, pk, j.M, j.M, NS_C * SP / (SA * SA));
+                t.e = c.a; t.beta = NS_B * SP / SA; t.gamma = NS_A * SP;
+                w.phase = w.run > 1 ? COLLECT : APPLY;
+                return;
+            }
+            case COLLECT:
+                if (w.k < w.run) add(SYMM, j, pk, c.a, c.r, j.M, j.M, 1.f / SP);
+                if (w.k > 1) add(SYMM, j, pk, w.k == 2 ? c.p0 : c.q0, w.k == 2 ? c.q0 : c.q1, j.M, j.M, SQ[w.k] / (SP * SQ[w.k - 1]));
+                w.phase = w.k < w.run ? NEXT : APPLY;
+                return;
+            case NEXT:
+                add(SYMM, j, pk, c.r, c.a, j.M, j.M, 1.f / SP);
+                ++w.k;
+                w.phase = POLY;
+                return;
+            default: {
+                const long q = w.run == 1 ? c.p0 : w.run == 2 ? c.q0 : c.q1;
+                Task& t = add(BOTH, j, q, w.odd ? c.xt1 : j.xt, j.x, j.N, j.M, 1.f / SQ[w.run]);
+                w.done += w.run;
+                if (w.done < steps) t.dt = w.odd ? j.xt : c.xt1;
+                else { t.d = (long)j.out; t.alpha /= SX; t.rows = j.rows; t.cols = j.cols; t.tall = j.tall; }
+                w.odd = !w.odd;
+                w.phase = w.done < steps ? GRAM : END;
+            }
         }
-        done += run;
-        LEVEL(const long q = run == 1 ? c.p0 : run == 2 ? c.q0 : c.q1;
-              Task& t = add(done < steps ? BOTH : hyper ? WEIGHT : OUT, j, q, odd ? c.xt1 : j.xt, j.x, j.N, j.M, 1.f / SQ[run]);
-              if (done < steps) t.dt = odd ? j.xt : c.xt1;
-              else { t.d = (long)j.out; t.alpha /= SX; t.rows = j.rows; t.cols = j.cols; t.tall = j.tall; });
-        odd = !odd;
+    };
+    // A level: the next products of all jobs that stand before some without E; of those with E if there are none; of the last ones. Jobs
+    // of the same runs go in step, and five iterations in runs of one and of three share 17 levels.
+    for (;;) {
+        auto rank = [&](int kind) { return kind < 0 ? 3 : kind == SYMM || kind == BOTH ? 0 : kind == SYMM_E ? 1 : 2; };
+        int least = 3, kinds = 0;
+        for (int i = 0; i < s.n; ++i) least = min(least, rank(kind_of(i)));
+        if (least == 3) return 0;
+        L.n = 0;
+        for (int i = 0; i < s.n; ++i)
+            if (rank(kind_of(i)) == least) {
+                L.kind = kind_of(i);
+                kinds |= 1 << L.kind;
+                emit(i);
+            }
+        if (kinds == (1 << SYMM | 1 << BOTH)) L.kind = MIXED;
+        if (int rc = run_level(L, p.slabs, st)) return rc;
     }
-#undef LEVEL
-    return 0;
 }
 }  // namespace
 

@@ -770,8 +770,8 @@ int cpcsv_norm_residual_bwd(const void* x, const void* u, const void* gate, cons
 /* ---- orthogonalised updates (csrc/orth.hip) ----------------------------------------------------------------------------
  * Stands beside cpcsv_adam_step (reference trainer.py:212-220 uses Adam for every net): an optimiser for matrices.
  *   X = U / (|U|_F + eps), then `steps` times  A = X X^T, X <- a X + (b A + c A^2) X  with (a, b, c) = (3.4445, -4.7750, 2.0315),
- *   on the transpose where rows > cols. Two fp16 planes per operand (22 bits and a sign), fp32 sums: results are up to twice as far off as
- *   those of fp32 products for sides up to 128, the same from about 370, nearer for wide matrices. A matrix of zeros stays zero.
+ *   on the transpose where rows > cols. Two fp16 planes per operand (22 bits and a sign), fp32 sums: results are about as far off as those
+ *   of fp32 products (on average 0.3 to 1.5 times). A matrix of zeros stays zero.
  * dims   HOST array [njobs][2] of rows, cols (1..CPCSV_ORTH_MAX_SIDE each, the shorter one up to CPCSV_ORTH_MAX_MIN); njobs in 1..CPCSV_ORTH_JOBS matrices share each launch
  * ws     device workspace of cpcsv_orth_workspace(dims, njobs) bytes, 16-byte aligned, contents irrelevant before and after
  * cpcsv_orthogonalize: HOST arrays of device pointers g -> out [rows][cols], both dtype

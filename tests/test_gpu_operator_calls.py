@@ -284,6 +284,45 @@ def test_16_bit_results_are_the_fp32_results_rounded(rows, cols):
         assert torch.equal(orthogonalize(g), got)
 
 
+@pytest.mark.parametrize("kind", ["gauss", "strong"])
+@pytest.mark.parametrize("rows,cols", [(17, 23), (32, 32), (64, 64), (63, 124), (128, 128), (90, 500), (12, 700), (2048, 16)])
+def test_small_matrices_keep_the_accuracy_of_fp32(rows, cols, kind):
+    """Over twenty matrices, the mean distance from the 64-bit result is at most one and a half times that of the same iteration in fp32."""
+    from cpcsv.optim import orthogonalize
+    from tests.test_gpu_orth import iterate, spectrum
+    own = kernel = 0.0
+    for seed in range(20):
+        g = spectrum(rows, cols, kind, seed).cuda()
+        want = iterate(g, 5, 1e-7)
+        own += ((iterate(g, 5, 1e-7, torch.float32).double() - want).norm() / want.norm()).item()
+        kernel += ((orthogonalize(g).double() - want).norm() / want.norm()).item()
+    assert kernel <= 1.5 * own, (kernel / 20, own / 20)
+
+
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 5, 7])
+def test_matrices_of_all_aspects_share_a_step(steps):
+    """Near-square and wide matrices, whose iterations form X at different times, in one call: each with the bits that it has alone, and
+    the smaller ones within their distance from the 64-bit result."""
+    from cpcsv.optim import FusedMuon
+    from tests.test_gpu_orth import bound, iterate
+    shapes = [(60, 60), (70, 900), (300, 310), (1000, 40), (129, 700), (1600, 1700), (520, 8), (1030, 5000)]
+    gen = torch.Generator("cuda").manual_seed(steps)
+    w0, gs = ([torch.randn(s, generator=gen, device="cuda") for s in shapes] for _ in range(2))
+
+    def step(which):
+        ps = [torch.nn.Parameter(w0[i].clone()) for i in which]
+        for p, i in zip(ps, which):
+            p.grad = gs[i].clone()
+        FusedMuon(ps, lr=0.1, momentum=0.0, steps=steps).step()
+        return [p.detach() for p in ps]
+    together = step(range(len(shapes)))
+    assert all(torch.equal(a, b) for a, b in zip(together[::-1], step(range(len(shapes))[::-1])))
+    for i, (r, c) in enumerate(shapes):
+        assert torch.equal(together[i], step([i])[0]), shapes[i]
+        x = 0.1 * max(1.0, r / c) ** 0.5 * iterate(gs[i], steps, 1e-7)
+        assert (together[i].double() - (w0[i].double() - x)).norm() <= bound(shapes[i]) * 3.9 ** max(0, steps - 5) * x.norm() + 3 * 2.0 ** -24 * w0[i].norm(), shapes[i]
+
+
 def test_a_learning_rate_tensor_changed_in_place_is_followed():
     """lr may be a tensor, which schedulers change in place: each step and sync_lr() read its value."""
     from cpcsv.optim import FusedMuon
