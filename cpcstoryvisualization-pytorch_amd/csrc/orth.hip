@@ -10,7 +10,8 @@
 // two runs (3 + 2) cost 6 M^2 N + 14 M^3 instead of the 15 M^2 N + 5 M^3 of forming X each time (all M x M results are symmetric:
 // one triangle is computed): equal for square matrices, 2.5 times fewer operations for wide ones. But the Gram matrix holds squares, and
 // what is rounded off beside the largest is amplified with the smallest: in fp32 all five in one run are up to 25 times further off than
-// X formed each time, 3 + 2 at most twice. Runs of three are for matrices that are wide enough to gain by them (run_of).
+// X formed each time, 3 + 2 up to three times for small square matrices and twice for wide ones. Runs of three are for matrices that
+// are wide enough to gain by them (run_of).
 //
 // Precision. One product in bf16 per step leaves the result 1e-2 off on well conditioned gradients and 3e-1 on those with a few
 // strong directions: what is lost next to the large singular values is amplified by a^5 = 485 where they are small. The operands
